@@ -292,6 +292,78 @@ int tcc_balance_tasks_padded(const tcc_sw32_task* tasks, uint32_t task_count, co
 int tcc_spmm_launch_shape(uint32_t features, int variant, uint32_t* grid, uint32_t* threads, uint32_t* smem,
                           int* occupancy);
 
+/* ---------------------------------------------------------------------------------
+ * Dense operators on 8-bit blocks
+ *
+ * The dense half of a layer whose sparse half is the SpMM above: the quantizer to 8-bit floating
+ * point, the product of two such matrices, and the INT8 checkpoint of an activation with the two
+ * gradients that are computed from it. No counterpart in the reference.
+ *
+ * Blocks. A matrix [rows x cols] is cut into blocks of 128 columns of a row (block_rows = 1) or of
+ * 128 x 128 elements (block_rows = 128); the last blocks end with the matrix. A block has one
+ * scale 2^e, e the least exponent with absmax <= 2^e * L (L = 448 for e4m3, 57344 for e5m2, 127 for
+ * INT8; e >= -126; 2^0 for a block of zeros), and its elements are x * 2^-e rounded to nearest,
+ * ties to even. scales[row block][column block] holds e + 127 as a byte (E8M0), contiguous,
+ * ceil(cols / 128) bytes per row of blocks. A block that holds an infinity or NaN has the scale
+ * byte 255 (NaN) and elements NaN (INT8: 0), and all that is computed from it is NaN.
+ *
+ * Strides are row strides in elements, at least the row's width; elements of a row are adjacent.
+ * A size of 0 is allowed. The matrices of a call must not overlap, but for y == x and
+ * grad_x == grad_y with equal strides.
+ * --------------------------------------------------------------------------------- */
+
+typedef enum tcc_type { TCC_F32 = 0, TCC_BF16 = 1, TCC_F16 = 2, TCC_E4M3 = 3, TCC_E5M2 = 4 } tcc_type;
+typedef enum tcc_activation {
+    TCC_RELU = 0,
+    TCC_GELU = 1,      /* x Phi(x) */
+    TCC_GELU_TANH = 2, /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 */
+    TCC_SILU = 3,      /* x / (1 + exp(-x)) */
+    TCC_IDENTITY = 4   /* checkpoint only: keeps x, writes no y */
+} tcc_activation;
+typedef enum tcc_b_layout { TCC_B_NK = 0, TCC_B_KN = 1 } tcc_b_layout;
+
+/* q, scales = the blocks of x (fp32, bf16 or fp16) in e4m3 or e5m2. */
+int tcc_quantize_blocks_fp8(const void* x, int x_type, uint64_t x_stride, void* q, int q_type,
+                            uint64_t q_stride, uint8_t* scales, uint32_t rows, uint32_t cols,
+                            uint32_t block_rows, tcc_stream_t stream);
+
+/* output[m x n] = A B^T + bias with A [m x k] and B [n x k] (TCC_B_NK) or, for B stored as [k x n]
+ * (TCC_B_KN: the gradient of a layer's input, from the layer's own weights), A B + bias. Both
+ * operands are e4m3 or e5m2 blocks along k; a [k x n] operand has blocks of 128 x 128. The sum is
+ * accumulated in fp32 and rounded once to fp32, bf16 or fp16; bias (n floats) may be NULL. Fast
+ * where both operands' rows start on 16 bytes (base and stride multiples of 16); other alignments
+ * run on a slower kernel. */
+int tcc_matmul_fp8_blocks(const void* a, int a_type, uint64_t a_stride, const uint8_t* a_scales,
+                          uint32_t a_block_rows, const void* b, int b_type, uint64_t b_stride,
+                          const uint8_t* b_scales, uint32_t b_block_rows, int b_layout,
+                          const float* bias, void* output, int output_type, uint64_t output_stride,
+                          uint32_t m, uint32_t n, uint32_t k, tcc_stream_t stream);
+
+/* y = f(x) (fp32, bf16 or fp16, both of one type), and x kept as INT8 blocks of 128 columns of a
+ * row in q and scales. TCC_IDENTITY keeps x alone (y must be NULL). */
+int tcc_activation_checkpoint_int8(const void* x, uint64_t x_stride, void* y, uint64_t y_stride,
+                                   int type, int8_t* q, uint64_t q_stride, uint8_t* scales,
+                                   uint32_t rows, uint32_t cols, int activation, tcc_stream_t stream);
+
+/* grad_x = grad_y * f'(x^), x^ the values that the checkpoint stands for. ReLU's slope is 1 where
+ * x^ > 0: an x below half a step of its block was kept as 0 and passes no gradient. */
+int tcc_activation_backward_int8(const void* grad_y, uint64_t grad_y_stride, int type, const int8_t* q,
+                                 uint64_t q_stride, const uint8_t* scales, void* grad_x,
+                                 uint64_t grad_x_stride, uint32_t rows, uint32_t cols, int activation,
+                                 tcc_stream_t stream);
+
+/* grad_w[n x k] = grad_y^T x^ (accumulate != 0: added to grad_w), the weight gradient of a layer
+ * whose input [rows x k] was kept as INT8 blocks of 128 columns of a row, summed in fp32 over the
+ * rows of grad_y [rows x n] (fp32, bf16 or fp16). The workspace (16-byte aligned; its contents need
+ * no preparation and do not outlive the call) has the size that the function below gives, 0 where
+ * none is needed; calls that may overlap in time need one each. The result does not depend on
+ * timing: the same inputs give the same bits. */
+int tcc_weight_grad_int8_workspace_size(uint32_t rows, uint32_t n, uint32_t k, uint64_t* bytes);
+int tcc_weight_grad_int8(const void* grad_y, int type, uint64_t grad_y_stride, const int8_t* q,
+                         uint64_t q_stride, const uint8_t* scales, float* grad_w,
+                         uint64_t grad_w_stride, uint32_t rows, uint32_t n, uint32_t k, int accumulate,
+                         void* workspace, uint64_t workspace_bytes, tcc_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

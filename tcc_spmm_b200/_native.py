@@ -125,6 +125,19 @@ SIGNATURES = {
     "tcc_device_matrix_view": (C.c_int, [C.c_void_p, C.POINTER(Sw32DeviceView)]),
     "tcc_device_matrix_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "tcc_device_matrix_free": (None, [C.c_void_p]),
+    "tcc_quantize_blocks_fp8": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p,
+                                          C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "tcc_matmul_fp8_blocks": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_uint32, C.c_void_p, C.c_int,
+                                        C.c_uint64, C.c_void_p, C.c_uint32, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                        C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "tcc_activation_checkpoint_int8": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p,
+                                                 C.c_uint64, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p]),
+    "tcc_activation_backward_int8": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p,
+                                               C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p]),
+    "tcc_weight_grad_int8_workspace_size": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, u64p]),
+    "tcc_weight_grad_int8": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                       C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p, C.c_uint64,
+                                       C.c_void_p]),
 }
 
 # Failure-path test hooks of the library (exported, not declared in the public header).

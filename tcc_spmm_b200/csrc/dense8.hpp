@@ -1,0 +1,43 @@
+// Host-side pieces shared by the 8-bit block-scaled dense operators (blocks8.cu, matmul_fp8.cu,
+// weight_grad.cu): argument checks and the launch check.
+#pragma once
+#include "common.hpp"
+
+#include <cuda_runtime.h>
+
+namespace tcc {
+
+inline void checkCudaCall(cudaError_t s) {
+    if (s != cudaSuccess)
+        throw CudaError(cudaGetErrorString(s));
+}
+inline void require(bool ok, const char* message) {
+    if (!ok)
+        throw std::invalid_argument(message);
+}
+inline bool alignedTo(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// Whether every row of a matrix starts on `a` bytes.
+inline bool rowsAlignedTo(const void* p, uint64_t strideBytes, uintptr_t a) {
+    return alignedTo(p, a) && strideBytes % a == 0;
+}
+inline bool isFloatType(int t) { return t == TCC_F32 || t == TCC_BF16 || t == TCC_F16; }
+inline bool isFp8Type(int t) { return t == TCC_E4M3 || t == TCC_E5M2; }
+inline uint32_t typeBytes(int t) { return t == TCC_F32 ? 4 : (t == TCC_BF16 || t == TCC_F16) ? 2 : 1; }
+template <typename T> T ceilDiv(T a, T b) { return (a + b - 1) / b; }
+// The matrix's bytes do not reach over the end of the address space (rows, cols > 0).
+inline bool extentFits(uint64_t rows, uint64_t cols, uint64_t stride, uint64_t elementBytes) {
+    return stride <= (uint64_t(1) << 60) / elementBytes / rows && cols <= stride;
+}
+inline int multiprocessors() {
+    int device = 0, sms = 0;
+    checkCudaCall(cudaGetDevice(&device));
+    checkCudaCall(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    return sms;
+}
+
+// Status words of the dense kernels' bounded waits, merged into tcc_device_status. Each lives in
+// its kernels' translation unit.
+uint32_t matmulDeviceStatus(bool reset);
+uint32_t weightGradDeviceStatus(bool reset);
+
+} // namespace tcc
