@@ -1,7 +1,7 @@
 // Product of two 8-bit block-scaled matrices on sm_100a:
 //   Y[m, n] = sum over k of a[m, k] 2^ea[m, k / 128] * b[n, k] 2^eb[n, k / 128]  (+ bias[n])
 #include "dense8.cuh"
-#include "dense8.hpp"
+#include "dense8_tc.cuh"
 
 namespace tcc {
 namespace {
@@ -98,17 +98,410 @@ template <typename T> void launchGeneric(const Product& p) {
     checkCudaCall(cudaGetLastError());
 }
 
-void launchProduct(const Product& p) {
-    switch (p.outType) {
-    case TCC_F32: launchGeneric<float>(p); break;
-    case TCC_BF16: launchGeneric<__nv_bfloat16>(p); break;
-    default: launchGeneric<__half>(p); break;
+// ---- tensor cores -------------------------------------------------------------------------------
+// One CTA per SM computes tiles of 128 x BN outputs. A warp issues TMA copies of 128 bytes of k per
+// stage (128-byte swizzle); one thread issues tcgen05.mma kind::mxf8f6f4, whose E8M0 scales are the
+// blocks' own bytes: the hardware takes one scale per 32 elements of k, and a block's four groups
+// take the same one, so no scale is applied outside the tensor core and the sum over all of k stays
+// in one FP32 accumulator in tensor memory. Scales travel as words of four consecutive blocks per
+// row, loaded by a warp of their own, copied to tensor memory by the MMA thread and picked by the
+// byte selector of the instruction descriptor. Eight warps store finished tiles.
+template <int BN, bool KN> struct Tile {
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kAcc = BN == 256 ? 1 : 2;       // accumulators in tensor memory
+    static constexpr int kSlots = 4;                     // groups of four blocks' scales
+    static constexpr int kSlabs = 1 + (BN + 127) / 128;  // of 512 bytes: A's rows, B's rows
+    static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kScaleOff = kStages * kStageBytes;
+    static constexpr int kBarOff = kScaleOff + kSlots * kSlabs * 512;
+    // full, empty [kStages]; scaleFull, scaleEmpty [kSlots]; accFull, accEmpty [kAcc]; TMEM address
+    static constexpr int kBars = 2 * kStages + 2 * kSlots + 2 * kAcc;
+    static constexpr int kBytes = kBarOff + 8 * kBars + 16 + 1024; // + alignment to 1024
+    static constexpr int kScaleCols = 4 * kSlabs;
+    static constexpr int kCols = kAcc * BN + kSlots * kScaleCols;
+    static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+    static constexpr int kEpilogueWarps = 8;
+    static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
+    static constexpr int kThreads = 32 * 11;
+    static_assert(kCols <= 512 && kBytes <= 232448, "resources");
+    static_assert(!KN || BN >= 128, "rows of a [k, n] operand are copied 128 bytes at a time");
+};
+
+// Instruction descriptor of kind::mxf8f6f4 without the byte selectors: types (0 e4m3, 1 e5m2) in
+// bits 7-9 and 10-12, B MN-major in bit 16, N / 8 in bits 17-22, E8M0 scales in bit 23, M / 128 in
+// bits 27-28. The selectors are bits 29-30 (A) and 4-5 (B).
+__host__ __device__ constexpr uint32_t scaledIdesc(bool aE5m2, bool bE5m2, bool kn, uint32_t n) {
+    return (uint32_t(aE5m2) << 7) | (uint32_t(bE5m2) << 10) | (uint32_t(kn) << 16) | ((n >> 3) << 17) | (1u << 23) |
+           (1u << 27);
+}
+
+struct ScaleView {
+    const uint8_t* data;
+    uint32_t rows, rowShift; // rows of the operand; rows per block = 1 << rowShift
+    uint32_t width;          // bytes per row of scales
+    bool words;              // rows of scales start on 4 bytes
+};
+struct ProductArgs {
+    ScaleView a, b;
+    const float* bias;
+    void* out;
+    uint64_t outStride;
+    int outType, outAlign; // outAlign: 32, 16 or 0 bytes that every output row starts on
+    uint32_t m, n, k, tilesM, tilesN;
+    uint32_t idesc;
+};
+
+// Scale bytes of blocks 4g .. 4g + 3 of one row; 1.0 for rows and blocks outside.
+__device__ __forceinline__ uint32_t scaleWord(const ScaleView& s, uint64_t row, uint32_t g) {
+    if (row >= s.rows)
+        return 0x7F7F7F7Fu;
+    const uint8_t* p = s.data + (row >> s.rowShift) * s.width + 4 * g;
+    if (s.words)
+        return __ldg(reinterpret_cast<const uint32_t*>(p));
+    uint32_t w = 0x7F7F7F7Fu;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (4 * g + i < s.width)
+            w = (w & ~(0xFFu << (8 * i))) | (uint32_t(__ldg(p + i)) << (8 * i));
+    return w;
+}
+// The same for column n of a [k, n] operand with blocks of 128 x 128.
+__device__ __forceinline__ uint32_t scaleWordKn(const ScaleView& s, uint32_t kBlocks, uint32_t n, uint32_t g) {
+    uint32_t w = 0x7F7F7F7Fu;
+    const uint32_t c = min(n / kBlock, s.width - 1);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (4 * g + i < kBlocks)
+            w = (w & ~(0xFFu << (8 * i))) | (uint32_t(__ldg(s.data + uint64_t(4 * g + i) * s.width + c)) << (8 * i));
+    return w;
+}
+
+// Tiles in groups of 16 rows of tiles, so that the tiles in flight share operands in L2.
+__device__ __forceinline__ void tilePlace(const ProductArgs& p, uint32_t t, uint64_t& m0, uint32_t& n0, uint32_t bn) {
+    const uint32_t span = 16 * p.tilesN;
+    const uint32_t first = t / span * 16, local = t % span;
+    const uint32_t height = min(16u, p.tilesM - first);
+    m0 = uint64_t(first + local % height) * 128;
+    n0 = local / height * bn;
+}
+
+__device__ __forceinline__ void storeGlobal32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// 16 columns of one output row from column c on.
+template <typename T>
+__device__ __forceinline__ void storeColumns16(const ProductArgs& p, uint64_t row, uint32_t c, const uint32_t* acc) {
+    if (c >= p.n)
+        return;
+    T* out = static_cast<T*>(p.out) + row * p.outStride + c;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        v[i] = __uint_as_float(acc[i]) + (p.bias && c + i < p.n ? __ldg(p.bias + c + i) : 0.0f);
+    if (p.outAlign != 0 && c + 16 <= p.n) {
+        constexpr int kE = kPer16<T>;
+        uint4 w[16 / kE];
+#pragma unroll
+        for (int i = 0; i < 16 / kE; ++i) {
+            float part[kE];
+#pragma unroll
+            for (int e = 0; e < kE; ++e)
+                part[e] = v[kE * i + e];
+            w[i] = pack16<T>(part);
+        }
+        if (p.outAlign == 32) {
+#pragma unroll
+            for (int i = 0; i < 16 / kE; i += 2) {
+                const uint32_t u[8] = {w[i].x, w[i].y, w[i].z, w[i].w, w[i + 1].x, w[i + 1].y, w[i + 1].z, w[i + 1].w};
+                storeGlobal32(reinterpret_cast<uint4*>(out) + i, u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16 / kE; ++i)
+                reinterpret_cast<uint4*>(out)[i] = w[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (c + i < p.n)
+                out[i] = fromFloat<T>(v[i]);
     }
+}
+
+template <int BN, bool KN>
+__global__ void __launch_bounds__(Tile<BN, KN>::kThreads, 1)
+    productTiles(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const ProductArgs p) {
+    using L = Tile<BN, KN>;
+    extern __shared__ unsigned char smemRaw[];
+    const uint32_t base = (dev::smemAddr(smemRaw) + 1023u) & ~1023u;
+    unsigned char* smem = smemRaw + (base - dev::smemAddr(smemRaw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full = base + L::kBarOff, empty = full + 8 * L::kStages;
+    const uint32_t scaleFull = empty + 8 * L::kStages, scaleEmpty = scaleFull + 8 * L::kSlots;
+    const uint32_t accFull = scaleEmpty + 8 * L::kSlots, accEmpty = accFull + 8 * L::kAcc;
+    const uint32_t tmemSlot = accEmpty + 8 * L::kAcc;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; ++i)
+            dev::mbarInit(full + 8 * i, 1), dev::mbarInit(empty + 8 * i, 1);
+        for (int i = 0; i < L::kSlots; ++i)
+            dev::mbarInit(scaleFull + 8 * i, 1), dev::mbarInit(scaleEmpty + 8 * i, 1);
+        for (int i = 0; i < L::kAcc; ++i)
+            dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, L::kEpilogueWarps);
+        dev::fenceBarrierInit();
+    }
+    if (warp == L::kMmaWarp) {
+        dev::tmemAlloc(tmemSlot, L::kTmemCols);
+        dev::tmemRelinquish();
+    }
+    dev::tcFenceBefore();
+    __syncthreads();
+    dev::tcFenceAfter();
+    const uint32_t tmem = dev::ldsU32(tmemSlot);
+    const uint32_t scaleTmem = tmem + L::kAcc * BN;
+    const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, groups = (kBlocks + 3) / 4;
+    const uint32_t tiles = p.tilesM * p.tilesN;
+
+    if (warp == L::kTmaWarp) {
+        if (lane == 0) {
+            tmaPrefetchMap(&mapA);
+            tmaPrefetchMap(&mapB);
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                uint64_t m0;
+                uint32_t n0;
+                tilePlace(p, t, m0, n0, BN);
+                for (uint32_t kb = 0; kb < kBlocks; ++kb, ++it) {
+                    const uint32_t s = it % L::kStages, turn = it / L::kStages;
+                    if (turn != 0 && !waitPhase(empty + 8 * s, (turn - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t a = base + s * L::kStageBytes, b = a + L::kABytes;
+                    dev::mbarArriveExpectTx(full + 8 * s, L::kStageBytes);
+                    tmaLoad2d(a, &mapA, kb * kBlock, uint32_t(m0), full + 8 * s);
+                    if constexpr (KN) {
+#pragma unroll
+                        for (int j = 0; j < BN / 128; ++j)
+                            tmaLoad2d(b + j * 16384, &mapB, n0 + 128 * j, kb * kBlock, full + 8 * s);
+                    } else {
+                        tmaLoad2d(b, &mapB, kb * kBlock, n0, full + 8 * s);
+                    }
+                }
+            }
+            // After a wait that ran out, no copy may still be on its way when the CTA exits.
+            if (!ok)
+                for (uint32_t i = it < L::kStages ? 0 : it - L::kStages; i < it; ++i)
+                    waitPhase(full + 8 * (i % L::kStages), (i / L::kStages) & 1);
+        }
+        __syncwarp();
+    } else if (warp == L::kMmaWarp) {
+        if (lane == 0) {
+            uint32_t it = 0, group = 0, seq = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++seq) {
+                const uint32_t acc = seq % L::kAcc, accTurn = seq / L::kAcc;
+                if (accTurn != 0 && !waitPhase(accEmpty + 8 * acc, (accTurn - 1) & 1))
+                    break;
+                dev::tcFenceAfter();
+                const uint32_t d = tmem + acc * BN;
+                for (uint32_t kb = 0; kb < kBlocks; ++kb, ++it) {
+                    const uint32_t slot = group % L::kSlots;
+                    const uint32_t sa = scaleTmem + slot * L::kScaleCols, sb = sa + 4;
+                    if (kb % 4 == 0) {
+                        if (!waitPhase(scaleFull + 8 * slot, (group / L::kSlots) & 1)) {
+                            ok = false;
+                            break;
+                        }
+                        dev::tcFenceAfter();
+                        const uint32_t slab = base + L::kScaleOff + slot * L::kSlabs * 512;
+#pragma unroll
+                        for (int i = 0; i < L::kSlabs; ++i)
+                            tcCopyScales(sa + 4 * i, slabDesc(slab + 512 * i));
+                    }
+                    const uint32_t s = it % L::kStages;
+                    if (!waitPhase(full + 8 * s, (it / L::kStages) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    dev::tcFenceAfter();
+                    const uint32_t a = base + s * L::kStageBytes, b = a + L::kABytes;
+                    const uint64_t descA = swizzledDesc(a, 16, 1024);
+                    const uint64_t descB = KN ? swizzledDesc(b, 16384, 1024) : swizzledDesc(b, 16, 1024);
+                    const uint32_t idesc = p.idesc | ((kb % 4) << 29) | ((kb % 4) << 4);
+                    const uint32_t steps = min(4u, (p.k - kb * kBlock + 31) / 32);
+                    for (uint32_t j = 0; j < steps; ++j)
+                        mmaScaled8(d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
+                    dev::tcCommit(empty + 8 * s);
+                    if (kb % 4 == 3 || kb + 1 == kBlocks) {
+                        dev::tcCommit(scaleEmpty + 8 * slot);
+                        ++group;
+                    }
+                }
+                if (ok)
+                    dev::tcCommit(accFull + 8 * acc);
+            }
+        }
+        __syncwarp();
+    } else if (warp == L::kScaleWarp) {
+        // Lane i holds rows i, i + 32, i + 64 and i + 96 of a slab, 16 bytes in shared memory.
+        constexpr int kWords = 4 * L::kSlabs;
+        uint32_t w[kWords];
+        auto fetch = [&](uint32_t t, uint32_t g) {
+            uint64_t m0;
+            uint32_t n0;
+            tilePlace(p, t, m0, n0, BN);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                w[c] = scaleWord(p.a, m0 + 32 * c + lane, g);
+#pragma unroll
+            for (int c = 0; c < kWords - 4; ++c) {
+                if (32 * c >= BN)
+                    w[4 + c] = 0x7F7F7F7Fu;
+                else if constexpr (KN)
+                    w[4 + c] = scaleWordKn(p.b, kBlocks, n0 + 32 * c + lane, g);
+                else
+                    w[4 + c] = scaleWord(p.b, n0 + 32 * c + lane, g);
+            }
+        };
+        uint32_t group = 0;
+        bool ok = true;
+        if (blockIdx.x < tiles)
+            fetch(blockIdx.x, 0);
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            for (uint32_t g = 0; g < groups; ++g, ++group) {
+                const uint32_t slot = group % L::kSlots, turn = group / L::kSlots;
+                uint32_t held[kWords];
+#pragma unroll
+                for (int i = 0; i < kWords; ++i)
+                    held[i] = w[i];
+                if (g + 1 < groups) // the next words' loads run under this group's wait
+                    fetch(t, g + 1);
+                else if (uint64_t(t) + gridDim.x < tiles)
+                    fetch(t + gridDim.x, 0);
+                if (turn != 0 && !waitPhase(scaleEmpty + 8 * slot, (turn - 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                unsigned char* slab = smem + L::kScaleOff + slot * L::kSlabs * 512 + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < L::kSlabs; ++i)
+                    *reinterpret_cast<uint4*>(slab + 512 * i) =
+                        make_uint4(held[4 * i], held[4 * i + 1], held[4 * i + 2], held[4 * i + 3]);
+                dev::fenceProxyAsyncShared();
+                __syncwarp();
+                if (lane == 0)
+                    dev::mbarArrive(scaleFull + 8 * slot);
+            }
+    } else {
+        constexpr int kHalf = BN / 2; // columns per warp: two warps share a lane quarter
+        const uint32_t quarter = warp % 4, half = warp / 4;
+        uint32_t seq = 0;
+        for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, ++seq) {
+            const uint32_t acc = seq % L::kAcc;
+            if (!waitPhase(accFull + 8 * acc, (seq / L::kAcc) & 1))
+                break;
+            dev::tcFenceAfter();
+            uint64_t m0;
+            uint32_t n0;
+            tilePlace(p, t, m0, n0, BN);
+            const uint32_t from = tmem + acc * BN + half * kHalf + (quarter << 21); // lanes in bits 16-31
+            uint32_t r[kHalf];
+            if constexpr (kHalf == 16) {
+                dev::tcLoad32x32bx16(from, r);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kHalf / 32; ++i)
+                    tcLoad32x32bx32(from + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * i));
+            }
+            dev::tcWaitLd();
+            dev::tcFenceBefore();
+            __syncwarp();
+            if (lane == 0)
+                dev::mbarArrive(accEmpty + 8 * acc);
+            const uint64_t row = m0 + 32 * quarter + lane;
+            if (row < p.m) {
+#pragma unroll
+                for (int i = 0; i < kHalf / 16; ++i) {
+                    const uint32_t c = n0 + half * kHalf + 16 * i;
+                    if (p.outType == TCC_BF16)
+                        storeColumns16<__nv_bfloat16>(p, row, c, r + 16 * i);
+                    else if (p.outType == TCC_F32)
+                        storeColumns16<float>(p, row, c, r + 16 * i);
+                    else
+                        storeColumns16<__half>(p, row, c, r + 16 * i);
+                }
+            }
+        }
+    }
+    dev::tcFenceBefore();
+    __syncthreads();
+    dev::tcFenceAfter();
+    if (warp == L::kMmaWarp)
+        dev::tmemDealloc(tmem, L::kTmemCols);
+}
+
+ScaleView scaleView(const Operand& o, uint32_t rows, uint32_t width) {
+    return {o.scales, rows, o.rowShift, width, width % 4 == 0 && alignedTo(o.scales, 4)};
+}
+
+template <int BN, bool KN> void launchTiles(const Product& p) {
+    using L = Tile<BN, KN>;
+    const uint32_t kBlocks = ceilDiv(p.k, kBlock);
+    ProductArgs args{};
+    args.a = scaleView(p.a, p.m, kBlocks);
+    args.b = KN ? ScaleView{p.b.scales, p.k, 7, ceilDiv(p.n, kBlock), false} : scaleView(p.b, p.n, kBlocks);
+    args.bias = p.bias;
+    args.out = p.out;
+    args.outStride = p.outStride;
+    args.outType = p.outType;
+    const uint64_t rowBytes = p.outStride * typeBytes(p.outType);
+    args.outAlign = rowsAlignedTo(p.out, rowBytes, 32) ? 32 : rowsAlignedTo(p.out, rowBytes, 16) ? 16 : 0;
+    args.m = p.m, args.n = p.n, args.k = p.k;
+    args.tilesM = ceilDiv(p.m, 128u);
+    args.tilesN = ceilDiv<uint32_t>(p.n, BN);
+    require(uint64_t(args.tilesM) * args.tilesN <= 0x7FFFFFFFull, "too many output tiles for one call");
+    args.idesc = scaledIdesc(p.a.type == TCC_E5M2, p.b.type == TCC_E5M2, KN, BN);
+    const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUtensorMap mapA = tensorMap2d(p.a.data, u8, 1, p.m, p.k, p.a.stride, 128, 128);
+    const CUtensorMap mapB = KN ? tensorMap2d(p.b.data, u8, 1, p.k, p.n, p.b.stride, 128, 128)
+                                : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, BN, 128);
+    checkCudaCall(cudaFuncSetAttribute(productTiles<BN, KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    const uint32_t grid = std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors());
+    productTiles<BN, KN><<<grid, L::kThreads, L::kBytes, p.stream>>>(mapA, mapB, args);
+    checkCudaCall(cudaGetLastError());
+}
+
+void launchProduct(const Product& p) {
+    const bool tma = p.k != 0 && rowsAlignedTo(p.a.data, p.a.stride, 16) && rowsAlignedTo(p.b.data, p.b.stride, 16) &&
+                     p.a.stride < (1ull << 40) && p.b.stride < (1ull << 40) &&
+                     std::max({p.m, p.n, p.k}) <= 0x7FFFFF00u; // coordinates of a copy are signed
+    if (!tma) {
+        switch (p.outType) {
+        case TCC_F32: launchGeneric<float>(p); break;
+        case TCC_BF16: launchGeneric<__nv_bfloat16>(p); break;
+        default: launchGeneric<__half>(p); break;
+        }
+        return;
+    }
+    const uint64_t rowTiles = ceilDiv(p.m, 128u), sms = multiprocessors();
+    if (rowTiles * ceilDiv(p.n, 256u) >= sms && p.n > 128)
+        p.kn ? launchTiles<256, true>(p) : launchTiles<256, false>(p);
+    else if (p.kn || rowTiles * ceilDiv(p.n, 128u) >= sms)
+        p.kn ? launchTiles<128, true>(p) : launchTiles<128, false>(p);
+    else if (rowTiles * ceilDiv(p.n, 64u) >= sms)
+        launchTiles<64, false>(p);
+    else
+        launchTiles<32, false>(p);
 }
 
 } // namespace
 
-uint32_t matmulDeviceStatus(bool) { return 0; }
+uint32_t matmulDeviceStatus(bool reset) { return denseStatus(reset); }
 
 } // namespace tcc
 

@@ -19,6 +19,7 @@
 // Every wait is bounded (about two seconds of %globaltimer); a wait that runs out records a
 // status word (tcc_device_status) and the kernel returns without hanging.
 #include "common.hpp"
+#include "dense8.hpp"
 #include "spmm_generic.cuh"
 #include "spmm_persistent.cuh"
 #include "spmm_tmem8.cuh"
@@ -336,6 +337,8 @@ int tcc_device_status(uint32_t* status, int reset) {
         cudaError_t s = cudaDeviceSynchronize();
         if (s == cudaSuccess)
             s = cudaMemcpyFromSymbol(status, tcc::gDeviceStatus, sizeof(uint32_t));
+        if (s == cudaSuccess)
+            *status |= tcc::matmulDeviceStatus(reset != 0) | tcc::weightGradDeviceStatus(reset != 0);
         if (s == cudaSuccess && reset) {
             const uint32_t zero = 0;
             s = cudaMemcpyToSymbol(tcc::gDeviceStatus, &zero, sizeof(uint32_t));

@@ -116,6 +116,18 @@ def test_product(m, n, k, out, layout, aligned):
     assert T.device_status() == 0
 
 
+@pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("m,n,k", [(2500, 2100, 200), (2500, 1000, 300), (1000, 1217, 640), (9000, 128, 1152), (40000, 260, 128),
+                                   (20, 9000, 136), (700, 4000, 1030)])
+def test_product_many_tiles(m, n, k, layout):
+    """More output tiles than SMs, so that a CTA computes several in turn, at every width of tile."""
+    a, sa, b, sb, want, size = product_case(m, n, k, layout=layout, seed=m)
+    y = torch.full((m, n), float("nan"), device="cuda", dtype=torch.float32 if layout == "nk" else torch.bfloat16)
+    T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
+    check_product(y, want, size, k)
+    assert T.device_status() == 0
+
+
 @pytest.mark.parametrize("a_rows,b_rows", [(1, 1), (128, 1), (128, 128)])
 @pytest.mark.parametrize("a_kind,b_kind", [("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("m", [5, 40, 300])
