@@ -43,37 +43,44 @@ __device__ __forceinline__ Place placeOf(uint64_t blocks, uint32_t colBlocks) {
 }
 
 // One lane's share of a block of x: pieces of 16 bytes (kPer16 elements), piece i at column
-// kPer16 * (8 i + lane). Columns at or beyond `cols` read as zero.
+// kPer16 * (8 i + lane), as they were loaded. Columns at or beyond `left` read as zero.
 template <typename T> struct Share {
     static constexpr int kElems = kPer16<T>;
     static constexpr int kPieces = kBlock / kGroup / kElems;
-    float v[kPieces][kElems];
-    __device__ __forceinline__ uint32_t column(int i, uint32_t lane) const { return kElems * (kGroup * i + lane); }
+    uint4 raw[kPieces];
+    static __device__ __forceinline__ uint32_t column(int i, uint32_t lane) { return kElems * (kGroup * i + lane); }
     __device__ __forceinline__ void load(const T* row, uint32_t left, uint32_t lane, bool vector) {
+        if (vector && left >= kBlock) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + column(i, lane)));
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const uint32_t c = column(i, lane);
             if (vector && c + kElems <= left) {
-                unpack16<T>(__ldcs(reinterpret_cast<const uint4*>(row + c)), v[i]);
+                raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + c));
             } else {
+                float v[kElems];
 #pragma unroll
                 for (int e = 0; e < kElems; ++e)
-                    v[i][e] = c + e < left ? toFloat(row[c + e]) : 0.0f;
+                    v[e] = c + e < left ? toFloat(row[c + e]) : 0.0f;
+                raw[i] = pack16<T>(v); // exact: the values have type T
             }
         }
     }
-    __device__ __forceinline__ void store(T* row, uint32_t left, uint32_t lane, bool vector) const {
+    // Piece i of a row of T.
+    static __device__ __forceinline__ void store(T* row, int i, const float (&v)[kElems], uint32_t left, uint32_t lane,
+                                                 bool vector) {
+        const uint32_t c = column(i, lane);
+        if (vector && c + kElems <= left) {
+            __stcs(reinterpret_cast<uint4*>(row + c), pack16<T>(v));
+        } else {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const uint32_t c = column(i, lane);
-            if (vector && c + kElems <= left) {
-                __stcs(reinterpret_cast<uint4*>(row + c), pack16<T>(v[i]));
-            } else {
-#pragma unroll
-                for (int e = 0; e < kElems; ++e)
-                    if (c + e < left)
-                        row[c + e] = fromFloat<T>(v[i][e]);
-            }
+            for (int e = 0; e < kElems; ++e)
+                if (c + e < left)
+                    row[c + e] = fromFloat<T>(v[e]);
         }
     }
 };
@@ -108,9 +115,8 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < Share<T>::kPieces; ++i)
-#pragma unroll
-        for (int e = 0; e < Share<T>::kElems; ++e)
-            top = max(top, __float_as_uint(s.v[i][e]) & 0x7FFFFFFFu);
+        top = absmax16<T>(s.raw[i], top);
+    top = absmaxBits<T>(top);
 #pragma unroll
     for (int offset = kGroup / 2; offset > 0; offset >>= 1)
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
@@ -119,27 +125,27 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t byte = scaleByte<Q>(top);
     const float inverse = inverseScale(byte);
     uint8_t* qRow = q + p.row * qStride + p.col;
+    if (lane == 0)
+        scales[p.row * colBlocks + p.col / kBlock] = uint8_t(byte);
 #pragma unroll
     for (int i = 0; i < Share<T>::kPieces; ++i) {
         constexpr int kE = Share<T>::kElems;
+        float v[kE];
+        unpack16<T>(s.raw[i], v);
         uint32_t w[kE / 4];
 #pragma unroll
         for (int h = 0; h < kE / 4; ++h)
             w[h] = byte == 255u ? nanBytes<Q>()
-                                : quantize4<Q>(s.v[i][4 * h] * inverse, s.v[i][4 * h + 1] * inverse,
-                                               s.v[i][4 * h + 2] * inverse, s.v[i][4 * h + 3] * inverse);
-        const uint32_t c = s.column(i, lane);
+                                : quantize4<Q>(v[4 * h] * inverse, v[4 * h + 1] * inverse, v[4 * h + 2] * inverse,
+                                               v[4 * h + 3] * inverse);
+        const uint32_t c = Share<T>::column(i, lane);
         storeBytes<kE>(qRow + c, w, left > c ? left - c : 0u, vectorQ);
-    }
-    if (lane == 0)
-        scales[p.row * colBlocks + p.col / kBlock] = uint8_t(byte);
-    if constexpr (A != kNone) {
+        if constexpr (A != kNone) {
 #pragma unroll
-        for (int i = 0; i < Share<T>::kPieces; ++i)
-#pragma unroll
-            for (int e = 0; e < Share<T>::kElems; ++e)
-                s.v[i][e] = activation<A>(s.v[i][e]);
-        s.store(y + p.row * yStride + p.col, left, lane, vectorY);
+            for (int e = 0; e < kE; e += 2)
+                activation<A>(v[e], v[e + 1]);
+            Share<T>::store(y + p.row * yStride + p.col, i, v, left, lane, vectorY);
+        }
     }
 }
 
@@ -174,13 +180,9 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        float v[kE];
-        unpack16<T>(raw[i], v);
-#pragma unroll
-        for (int e = 0; e < kE; ++e)
-            top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-    }
+    for (int i = 0; i < kPasses; ++i)
+        top = absmax16<T>(raw[i], top);
+    top = absmaxBits<T>(top);
     __shared__ uint32_t tops[kThreads / 32];
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     if (threadIdx.x % 32 == 0)
@@ -248,11 +250,18 @@ __global__ void __launch_bounds__(kThreads)
     Share<T> s;
     s.load(dy + p.row * dyStride + p.col, left, lane, vectorDy);
 #pragma unroll
-    for (int i = 0; i < Share<T>::kPieces; ++i)
+    for (int i = 0; i < Share<T>::kPieces; ++i) {
+        float v[kE];
+        unpack16<T>(s.raw[i], v);
 #pragma unroll
-        for (int e = 0; e < kE; ++e)
-            s.v[i][e] *= activationSlope<A>(int8At(w[i][e / 4], e % 4) * scale);
-    s.store(dx + p.row * dxStride + p.col, left, lane, vectorDx);
+        for (int e = 0; e < kE; e += 2) {
+            const uint32_t flipped = w[i][e / 4] ^ 0x80808080u;
+            float f = int8At(flipped, e % 4) * scale, g = int8At(flipped, e % 4 + 1) * scale;
+            activationSlope<A>(f, g);
+            v[e] *= f, v[e + 1] *= g;
+        }
+        Share<T>::store(dx + p.row * dxStride + p.col, i, v, left, lane, vectorDx);
+    }
 }
 
 uint32_t rowGrid(uint64_t blocks) {

@@ -28,6 +28,9 @@ template <> __device__ __forceinline__ float fromFloat<float>(float v) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 fromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half fromFloat<__half>(float v) { return __float2half_rn(v); }
 
+template <typename T> constexpr bool isHalf = false;
+template <> constexpr bool isHalf<__half> = true;
+
 // 16 bytes of T as floats, and back.
 template <typename T> constexpr int kPer16 = 16 / int(sizeof(T));
 template <typename T> __device__ __forceinline__ void unpack16(uint4 w, float (&v)[kPer16<T>]);
@@ -73,6 +76,25 @@ template <> __device__ __forceinline__ uint4 pack16<__half>(const float (&v)[8])
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// Running absmax of 16 bytes of T as unsigned words, and its final value as the bits of a float. The
+// 16-bit types compare two elements at a time in their own bits, which order as the floats do.
+template <typename T> __device__ __forceinline__ uint32_t absmax16(uint4 w, uint32_t top) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(max(top, w.x & 0x7FFFFFFFu), max(w.y & 0x7FFFFFFFu, w.z & 0x7FFFFFFFu)), w.w & 0x7FFFFFFFu);
+    } else {
+        constexpr uint32_t m = 0x7FFF7FFFu;
+        return __vmaxu2(__vmaxu2(top, w.x & m), __vmaxu2(__vmaxu2(w.y & m, w.z & m), w.w & m));
+    }
+}
+template <typename T> __device__ __forceinline__ uint32_t absmaxBits(uint32_t top) {
+    if constexpr (sizeof(T) == 4)
+        return top;
+    const uint32_t h = max(top & 0xFFFFu, top >> 16);
+    if constexpr (sizeof(T) == 2 && !isHalf<T>)
+        return h << 16;
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+}
+
 // ---- scale of a block -------------------------------------------------------------------------
 // The scale byte from the bits of the block's absmax (compared as unsigned integers, which order
 // non-negative floats, infinity and NaN). largest = 1.75 * 2^8 (E4M3), 1.75 * 2^15 (E5M2) or
@@ -111,44 +133,106 @@ template <int Q> __device__ __forceinline__ uint32_t quantize4(float a, float b,
 // The bytes of a block whose scale is NaN.
 template <int Q> __device__ __forceinline__ uint32_t nanBytes() { return Q == kInt8 ? 0u : 0x7F7F7F7Fu; }
 
-__device__ __forceinline__ float int8At(uint32_t word, int i) { return float(int8_t(word >> (8 * i))); }
+// Byte i of a word of INT8 elements that were flipped to unsigned (word ^ 0x80808080) as a float: the
+// byte under the exponent of 2^23, minus 2^23 + 128 (exact; no conversion instruction).
+__device__ __forceinline__ float int8At(uint32_t flipped, int i) {
+    return __uint_as_float(__byte_perm(flipped, 0x4B000000u, 0x7540 + i)) - 8388736.0f;
+}
 
 // ---- activation functions -----------------------------------------------------------------------
-// Phi(x) = erfc(-x / sqrt 2) / 2 and the logistic forms keep the relative accuracy of the left tail,
-// which 1 + erf and 1 + tanh lose.
-__device__ __forceinline__ float normalCdf(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
+// All forms keep the relative accuracy of the left tail, which 1 + erf and 1 + tanh lose. They work
+// on pairs, with the packed FP32 instructions (two lanes per issue) where there is a polynomial.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    return (uint64_t(__float_as_uint(b)) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float2 unpair2(uint64_t v) {
+    return make_float2(__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32)));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// The hardware's approximations (2^-22 relative), results below 2^-126 as zero: without the steps
+// that keep subnormal results, which no rounding of the outputs could show.
+__device__ __forceinline__ float exp2Approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocalApprox(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The normal distribution's tail Phi(-|x|) and its density's factor exp(-x^2 / 2), of two values.
+// Phi(-a) exp(a^2 / 2) is a smooth function of t = 1 / (1 + 0.3 a): t times a polynomial of degree 7
+// fitted to the least largest relative error over 0 <= a <= 14 (1.5e-7; 5e-7 with fp32 arithmetic).
+// Beyond a = 16 both are below the smallest float.
+struct Tail {
+    float2 phi, density;
+};
+__device__ __forceinline__ Tail normalTail(float x0, float x1) {
+    const float a0 = fminf(fabsf(x0), 16.0f), a1 = fminf(fabsf(x1), 16.0f);
+    const uint64_t a = pair2(a0, a1);
+    const float2 d = unpair2(fma2(a, pair2(0.3f, 0.3f), pair2(1.0f, 1.0f)));
+    const uint64_t t = pair2(reciprocalApprox(d.x), reciprocalApprox(d.y));
+    const float c[8] = {0.11962928622961044f, 0.12075415253639221f, 0.09991224855184555f, 0.1285656988620758f,
+                        -0.053691279143095016f, 0.20636169612407684f, -0.15720775723457336f, 0.03567587584257126f};
+    uint64_t s = pair2(c[7], c[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i)
+        s = fma2(s, t, pair2(c[i], c[i]));
+    const float2 e = unpair2(mul2(mul2(a, a), pair2(-0.72134752044448170f, -0.72134752044448170f))); // -log2(e) / 2
+    const uint64_t density = pair2(exp2Approx(e.x), exp2Approx(e.y));
+    return {unpair2(mul2(mul2(s, t), density)), unpair2(density)};
+}
+
 // 1 / (1 + exp(-x)) by exp(-|x|), so that the divisor stays within [1, 2] and nothing overflows.
 __device__ __forceinline__ float logistic(float x) {
-    const float t = __expf(-fabsf(x));
-    return __fdividef(x < 0.0f ? t : 1.0f, 1.0f + t);
+    const float t = exp2Approx(-1.4426950408889634f * fabsf(x));
+    return (x < 0.0f ? t : 1.0f) * reciprocalApprox(1.0f + t);
 }
 __device__ __forceinline__ float tanhArgument(float x) { // 2 sqrt(2/pi) (x + 0.044715 x^3)
     return x * (1.5957691216057308f + 0.0713548162726009f * x * x);
 }
 
-template <int A> __device__ __forceinline__ float activation(float x) {
-    if constexpr (A == kRelu)
-        return x < 0.0f ? 0.0f : x;
-    else if constexpr (A == kGelu)
-        return x * normalCdf(x);
-    else if constexpr (A == kGeluTanh)
-        return x * logistic(tanhArgument(x));
-    else if constexpr (A == kSilu)
-        return x * logistic(x);
-    else
-        return x;
-}
-template <int A> __device__ __forceinline__ float activationSlope(float x) {
+// f of two values, in place.
+template <int A> __device__ __forceinline__ void activation(float& x, float& y) {
     if constexpr (A == kRelu) {
-        return x > 0.0f ? 1.0f : x == x ? 0.0f : x;
-    } else if constexpr (A == kGelu) {
-        return normalCdf(x) + x * 0.3989422804014327f * __expf(-0.5f * x * x);
+        x = x < 0.0f ? 0.0f : x, y = y < 0.0f ? 0.0f : y;
+    } else if constexpr (A == kGelu) { // max(x, 0) - |x| Phi(-|x|)
+        const Tail t = normalTail(x, y);
+        x = (x < 0.0f ? 0.0f : x) - fminf(fabsf(x), 16.0f) * t.phi.x;
+        y = (y < 0.0f ? 0.0f : y) - fminf(fabsf(y), 16.0f) * t.phi.y;
     } else if constexpr (A == kGeluTanh) {
-        const float s = logistic(tanhArgument(x));
-        return s + x * s * (1.0f - s) * (1.5957691216057308f + 0.2140644488178027f * x * x);
+        x *= logistic(tanhArgument(x)), y *= logistic(tanhArgument(y));
+    } else if constexpr (A == kSilu) {
+        x *= logistic(x), y *= logistic(y);
+    }
+}
+// f' of two values, in place.
+template <int A> __device__ __forceinline__ void activationSlope(float& x, float& y) {
+    if constexpr (A == kRelu) {
+        x = x > 0.0f ? 1.0f : x == x ? 0.0f : x, y = y > 0.0f ? 1.0f : y == y ? 0.0f : y;
+    } else if constexpr (A == kGelu) { // Phi(x) + x phi(x)
+        const Tail t = normalTail(x, y);
+        x = (x < 0.0f ? t.phi.x : 1.0f - t.phi.x) + x * (0.3989422804014327f * t.density.x);
+        y = (y < 0.0f ? t.phi.y : 1.0f - t.phi.y) + y * (0.3989422804014327f * t.density.y);
+    } else if constexpr (A == kGeluTanh) {
+        const float s = logistic(tanhArgument(x)), u = logistic(tanhArgument(y));
+        x = s + x * s * (1.0f - s) * (1.5957691216057308f + 0.2140644488178027f * x * x);
+        y = u + y * u * (1.0f - u) * (1.5957691216057308f + 0.2140644488178027f * y * y);
     } else {
-        const float s = logistic(x);
-        return s + x * s * (1.0f - s);
+        const float s = logistic(x), u = logistic(y);
+        x = s + x * s * (1.0f - s), y = u + y * u * (1.0f - u);
     }
 }
 

@@ -3,6 +3,8 @@
 #pragma once
 #include "common.hpp"
 
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 namespace tcc {
@@ -28,11 +30,32 @@ template <typename T> T ceilDiv(T a, T b) { return (a + b - 1) / b; }
 inline bool extentFits(uint64_t rows, uint64_t cols, uint64_t stride, uint64_t elementBytes) {
     return stride <= (uint64_t(1) << 60) / elementBytes / rows && cols <= stride;
 }
-inline int multiprocessors() {
-    int device = 0, sms = 0;
+inline int currentDevice() {
+    int device = 0;
     checkCudaCall(cudaGetDevice(&device));
-    checkCudaCall(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    return device;
+}
+// Multiprocessors of the current device (asked once per device).
+inline int multiprocessors() {
+    static std::atomic<int> known[64] = {};
+    const int device = currentDevice();
+    int sms = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (sms == 0) {
+        checkCudaCall(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+        if (device < 64)
+            known[device].store(sms, std::memory_order_relaxed);
+    }
     return sms;
+}
+// Lets a kernel use `bytes` of dynamic shared memory on the current device (set once per device).
+template <auto Kernel> void allowSharedMemory(int bytes) {
+    static std::atomic<bool> done[64] = {};
+    const int device = currentDevice();
+    if (device < 64 && done[device].load(std::memory_order_acquire))
+        return;
+    checkCudaCall(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (device < 64)
+        done[device].store(true, std::memory_order_release);
 }
 
 // Status words of the dense kernels' bounded waits, merged into tcc_device_status. Each lives in

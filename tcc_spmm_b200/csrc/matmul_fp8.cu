@@ -470,7 +470,7 @@ template <int BN, bool KN> void launchTiles(const Product& p) {
     const CUtensorMap mapA = tensorMap2d(p.a.data, u8, 1, p.m, p.k, p.a.stride, 128, 128);
     const CUtensorMap mapB = KN ? tensorMap2d(p.b.data, u8, 1, p.k, p.n, p.b.stride, 128, 128)
                                 : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, BN, 128);
-    checkCudaCall(cudaFuncSetAttribute(productTiles<BN, KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    allowSharedMemory<productTiles<BN, KN>>(L::kBytes);
     const uint32_t grid = std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors());
     productTiles<BN, KN><<<grid, L::kThreads, L::kBytes, p.stream>>>(mapA, mapB, args);
     checkCudaCall(cudaGetLastError());

@@ -466,7 +466,7 @@ template <typename T, int BK> void launchTiles(const GradArgs& g, const Plan& p,
     using L = GradTile<T, BK>;
     const uint64_t grid = uint64_t(p.tilesN) * p.tilesK * p.splits;
     require(grid <= 0x7FFFFFFFull, "too many output tiles for one call");
-    checkCudaCall(cudaFuncSetAttribute(gradTiles<T, BK>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    allowSharedMemory<gradTiles<T, BK>>(L::kBytes);
     gradTiles<T, BK><<<uint32_t(grid), L::kThreads, L::kBytes, stream>>>(g);
     checkCudaCall(cudaGetLastError());
     if (p.splits > 1) {

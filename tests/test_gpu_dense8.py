@@ -214,9 +214,9 @@ def test_checkpoint_and_backward(rows, cols, dtype, kind):
         assert torch.equal(scales, want_scales) and same(q, want_q)
         want = D.activation(x.double(), kind)
         off = (y.double() - want).abs()
-        assert (off <= (function_bound(x.double(), kind) + D.half_step(dt)) * want.abs() + 2.0 ** -24).all() if \
-            dt == torch.float16 else \
-            (off <= (function_bound(x.double(), kind) + D.half_step(dt)) * want.abs() + 2.0 ** -120).all()
+        # an exponential below 2^-126 counts as zero: less than |x| 2^-126 of y; and the type's own smallest step
+        least = x.double().abs() * 2.0 ** -126 + (2.0 ** -24 if dt == torch.float16 else 2.0 ** -120)
+        assert (off <= (function_bound(x.double(), kind) + D.half_step(dt)) * want.abs() + least).all()
 
         T.activation_backward_int8(dy, q, scales, dx, activation=kind)
         xh = D.values(q, scales)
