@@ -88,9 +88,100 @@ __device__ __forceinline__ void tcLoad32x32bx32(uint32_t taddr, uint32_t (&r)[32
                  : "memory");
 }
 
-// A 2-D map of rows x cols bytes-or-wider elements with the 128-byte swizzle and zeros outside.
+// ---- clusters of one or two CTAs (CG) ----------------------------------------------------------
+__device__ __forceinline__ uint32_t clusterRank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// All threads of the CTAs of the cluster.
+template <int CG> __device__ __forceinline__ void clusterSync() {
+    if constexpr (CG == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+// Arrive on the barrier at this address of the cluster's first CTA.
+template <int CG> __device__ __forceinline__ void arriveLeader(uint32_t bar) {
+    if constexpr (CG == 1)
+        dev::mbarArrive(bar);
+    else
+        asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+                     "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+                     : "memory");
+}
+// waitPhase for a barrier on which the other CTA of the cluster arrives too.
+template <int CG> __device__ __forceinline__ bool waitCluster(uint32_t bar, uint32_t parity) {
+    if constexpr (CG == 1)
+        return waitPhase(bar, parity);
+    uint64_t start = 0;
+    for (uint32_t attempt = 1;; ++attempt) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done)
+                     : "r"(bar), "r"(parity), "r"(2000u)
+                     : "memory");
+        if (done)
+            return true;
+        if ((attempt & 63u) == 0) {
+            const uint64_t now = dev::globalTimerNs();
+            if (start == 0) {
+                start = now;
+            } else if (now - start > kDenseWaitNs) {
+                atomicOr(&gDenseStatus, 1u);
+                return false;
+            }
+        }
+    }
+}
+// One arrival on the barrier at this address in every CTA of the cluster, once the tcgen05
+// operations that this thread issued are done.
+template <int CG> __device__ __forceinline__ void commitCluster(uint32_t bar) {
+    if constexpr (CG == 1)
+        dev::tcCommit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(static_cast<unsigned short>(3))
+                     : "memory");
+}
+template <int CG> __device__ __forceinline__ void tmemAllocGroup(uint32_t dst, uint32_t cols) {
+    if constexpr (CG == 1) {
+        dev::tmemAlloc(dst, cols);
+        dev::tmemRelinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG> __device__ __forceinline__ void tmemDeallocGroup(uint32_t taddr, uint32_t cols) {
+    if constexpr (CG == 1)
+        dev::tmemDealloc(taddr, cols);
+    else
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
+// Warp store of 16 TMEM lanes x 8 columns: thread t writes lane t / 4 (r0, r1) and lane t / 4 + 8
+// (r2, r3) at columns 2 (t % 4) and 2 (t % 4) + 1.
+__device__ __forceinline__ void tcStore16x256b(uint32_t taddr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r0), "r"(r1), "r"(r2),
+                 "r"(r3)
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void registersUp() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void registersDown() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// A 2-D map of rows x cols bytes-or-wider elements and zeros outside, swizzled unless told otherwise.
 inline CUtensorMap tensorMap2d(const void* base, CUtensorMapDataType type, uint32_t elementBytes, uint64_t rows,
-                               uint64_t cols, uint64_t stride, uint32_t boxRows, uint32_t boxCols) {
+                               uint64_t cols, uint64_t stride, uint32_t boxRows, uint32_t boxCols,
+                               CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -107,7 +198,7 @@ inline CUtensorMap tensorMap2d(const void* base, CUtensorMapDataType type, uint3
     const cuuint64_t strides[1] = {stride * elementBytes};
     const cuuint32_t box[2] = {boxCols, boxRows}, steps[2] = {1, 1};
     if (encode(&map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
+               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
         CUDA_SUCCESS)
         throw CudaError("cuTensorMapEncodeTiled refused a matrix");
     return map;

@@ -6,12 +6,21 @@
 // split into P bf16 parts that add up to it (P = 1 for bf16, 2 for fp16: 8 + 3 bits, 3 for fp32:
 // 8 + 8 + 8 bits), each multiplied on its own into the same accumulator.
 //
-// A CTA computes 128 rows of dW (n) by BK columns (k) over a range of rows r. dy^T is operand A in
-// tensor memory: a thread loads four neighbouring columns of a row at a time and pairs rows with
-// byte permutes, so A never passes through shared memory, whose bandwidth the B side needs. q^ is
-// operand B in shared memory, row-major as it comes (MN-major, 128-byte swizzle), converted on the
-// way by warps of their own. Two sets of producer warps take alternate stages, so the global loads
-// of one run under the conversions of the other; one thread issues the MMAs.
+// A cluster of CG CTAs computes 128 CG rows (n) by 256 columns (k) of dW over a range of rows r, with
+// tcgen05.mma over the pair where CG = 2: each CTA brings 128 columns of dy and half of the columns
+// of q^, which halves the conversions and the shared-memory reads of an SM. CG = 1 where dW has at
+// most 128 rows.
+//
+// Raw rows arrive by TMA in a ring of stages. Four warps turn dy into operand A in tensor memory: a
+// thread takes four neighbouring columns of a row at a time and pairs rows with byte permutes. Four
+// warps turn q into operand B in shared memory, row-major as it comes (MN-major, 128-byte swizzle).
+// One thread issues the MMAs.
+//
+// The tensor core cuts off what an addition shifts out below the accumulator's last bit, about
+// 1.5e-8 of the sum for every MMA (measured; 2.1e-5 after 1300), so the accumulator is emptied every
+// kFlush MMAs into fp32 registers, which round to nearest. The two halves of the 256 columns take
+// turns, half a period apart, over three accumulators of 128 columns: the MMAs go on in the third
+// while eight warps read one out.
 #include "dense8.cuh"
 #include "dense8_tc.cuh"
 
@@ -30,71 +39,73 @@ struct GradArgs {
     const uint8_t* scales;
     float* dw;
     uint64_t dwStride;
-    float* partials; // [split][tile][BK / 4][128][4], null when the rows are not split
+    float* partials; // [split][tile][CTA][64][128][4], null when the rows are not split
     uint32_t rows, n, k;
     uint32_t tilesN, tilesK, rowsPerSplit;
-    bool accumulate, vectorDy, vectorQ;
-    int dwAlign; // 32, 16 or 0 bytes that every row of dw starts on
+    bool accumulate;
+    bool dwVector; // rows of dw start on 16 bytes
 };
 
 template <typename T> constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
 template <> constexpr int kParts<__half> = 2;
 
-template <typename T, int BK> struct GradTile {
+template <typename T, int CG> struct GradTile {
     static constexpr int kP = kParts<T>;
-    static constexpr int kRows = kP == 3 ? 32 : 64; // rows per stage
-    static constexpr int kStages = 4;
-    static constexpr int kBBytes = kRows * BK * 2;
-    static constexpr int kACols = kP * kRows / 2;   // tensor-memory columns of a stage of A
-    static constexpr int kBarOff = kStages * kBBytes;
-    static constexpr int kNeed = kBarOff + 8 * (2 * kStages + 1) + 16 + 1024;
-    // At least half of the shared memory: a second CTA on the SM would wait for tensor memory.
-    static constexpr int kBytes = kNeed > 120 * 1024 ? kNeed : 120 * 1024;
-    static constexpr int kCols = BK + kStages * kACols;
-    static constexpr int kTmemCols = kCols <= 256 ? 256 : 512;
-    static constexpr int kAWarps = 8, kBWarps = 8, kMmaWarp = 16;
-    static constexpr int kThreads = 32 * 17;
-    static_assert(kCols <= 512 && kBytes <= 232448, "resources");
+    static constexpr int kRows = kP == 3 ? 32 : 64;    // rows per stage
+    static constexpr int kBk = 256, kBCols = kBk / CG; // columns of dW: of the cluster, of q in this CTA
+    static constexpr int kRaw = CG == 1 && kP < 3 ? 3 : 6, kStages = kP == 1 ? 3 : 2;
+    static constexpr int kABoxes = int(sizeof(T)), kBBoxes = kBCols / 128; // of 128 bytes x kRows
+    static constexpr int kBox = kRows * 128;
+    static constexpr int kRawBytes = (kABoxes + kBBoxes) * kBox;
+    static constexpr int kBBytes = kRows * kBCols * 2;
+    static constexpr int kACols = kP * kRows / 2;       // tensor-memory columns of a stage of A
+    static constexpr int kSteps = kP * kRows / 16;      // MMAs per stage and accumulator
+    static constexpr int kFlush = 60 / kSteps / 2 * 2;  // stages between two flushes of a half (even)
+    static constexpr int kRawOff = kStages * kBBytes;
+    static constexpr int kBarOff = kRawOff + kRaw * kRawBytes;
+    // rawFull, rawEmpty [kRaw]; full, empty [kStages]; accFull, accEmpty [2]; TMEM address
+    static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 2 * kStages + 4) + 16 + 1024;
+    static constexpr int kCols = 3 * 128 + kStages * kACols;
+    static constexpr int kEpilogueWarps = 8, kBWarp = 12, kLoadWarp = 16, kMmaWarp = 19;
+    static constexpr int kThreads = 32 * 20;
+    // Registers: 96 per thread at launch; the warpgroups then share them out, 168 for the epilogue's
+    // 128 sums.
+    static constexpr int kRegs = 96, kRegsEpilogue = 168, kRegsConvert = 56, kRegsIssue = 32;
+    static_assert(2 * kRegsEpilogue + 2 * kRegsConvert + kRegsIssue <= 5 * kRegs, "the shares exceed the launch's registers");
+    static_assert(kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
+    static_assert(kFlush >= 2 && kFlush % 2 == 0, "flush period");
 };
 
 // kind::f16 with FP32 accumulators (bits 4-5 = 1), bf16 A and B (bits 7-9 and 10-12 = 1), B
 // MN-major (bit 16), N / 8 in bits 17-22 and M / 16 in bits 24-28.
-__host__ __device__ constexpr uint32_t bf16Idesc(uint32_t n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+__host__ __device__ constexpr uint32_t bf16Idesc(uint32_t m, uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 // D(tmem) (+)= A(tmem, bf16) x B(shared memory, bf16).
+template <int CG>
 __device__ __forceinline__ void mmaBf16Ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
 }
 
-// Four neighbouring columns of one row of dy, as loaded.
+// Four neighbouring columns of one row of dy, from a raw stage.
 template <typename T> struct Quad { uint32_t w[sizeof(T)]; };
-
-template <typename T> __device__ __forceinline__ Quad<T> loadQuad(const T* p, uint32_t left, bool vector) {
+template <typename T> __device__ __forceinline__ Quad<T> loadQuad(uint32_t addr) {
     Quad<T> v;
-    if (vector && left >= 4) {
-        if constexpr (sizeof(T) == 4) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-            v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
-        } else {
-            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-            v.w[0] = u.x, v.w[1] = u.y;
-        }
+    if constexpr (sizeof(T) == 4) {
+        const uint4 u = dev::ldsV4(addr);
+        v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
     } else {
-        const uint32_t zero = 0;
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T)); ++i) {
-            if constexpr (sizeof(T) == 4) {
-                v.w[i] = uint32_t(i) < left ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : zero;
-            } else {
-                const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-                v.w[i] = (uint32_t(2 * i) < left ? uint32_t(__ldg(h + 2 * i)) : zero) |
-                         (uint32_t(2 * i + 1) < left ? uint32_t(__ldg(h + 2 * i + 1)) << 16 : zero);
-            }
-        }
+        const uint2 u = dev::ldsV2(addr);
+        v.w[0] = u.x, v.w[1] = u.y;
     }
     return v;
 }
@@ -161,245 +172,349 @@ __device__ __forceinline__ __nv_bfloat162 scalePair(uint32_t byte) {
 // half of the quarter takes columns 0 and 1 of each four, the second half 2 and 3.
 __device__ __forceinline__ uint32_t laneColumn(uint32_t l) { return 4 * (l % 8) + 2 * (l / 16) + (l / 8) % 2; }
 
-template <int REPEAT> __device__ __forceinline__ void storeA(uint32_t taddr, const uint32_t (&r)[4 * REPEAT]) {
-    if constexpr (REPEAT == 4)
-        dev::tcStore16x256bx4(taddr, r);
-    else
-        dev::tcStore16x256bx2(taddr, r);
+// Column of dW (from the tile's first) of column c of the accumulator half h. Over a pair of CTAs an
+// MMA takes its first columns from the first CTA's shared memory, the others from the second's.
+template <int CG> __device__ __forceinline__ uint32_t columnOf(uint32_t h, uint32_t c) {
+    return CG == 1 ? 128 * h + c : 64 * h + c % 64 + c / 64 * 128;
 }
 
-template <typename T, int BK>
-__global__ void __launch_bounds__(GradTile<T, BK>::kThreads, 1) gradTiles(const GradArgs p) {
-    using L = GradTile<T, BK>;
+// Row of a raw stage whose values stand at row k of the operands. Any order will do that A and B
+// share; this one lets the four threads that read one column group of dy take rows two apart, which
+// the TMA swizzle puts into distinct banks.
+__device__ __forceinline__ uint32_t operandRow(uint32_t r) { // its inverse: raw row -> operand row
+    return (r & ~15u) | ((r & 6u) << 1) | ((r & 8u) >> 2) | (r & 1u);
+}
+
+template <typename T, int CG, bool TMA>
+__global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
+    gradTiles(const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ CUtensorMap mapQ, const GradArgs p) {
+    using L = GradTile<T, CG>;
     extern __shared__ unsigned char smemRaw[];
     const uint32_t base = (dev::smemAddr(smemRaw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full = base + L::kBarOff, empty = full + 8 * L::kStages, done = empty + 8 * L::kStages;
-    const uint32_t tmemSlot = done + 8;
+    const uint32_t rawFull = base + L::kBarOff, rawEmpty = rawFull + 8 * L::kRaw;
+    const uint32_t full = rawEmpty + 8 * L::kRaw, empty = full + 8 * L::kStages;
+    const uint32_t accFull = empty + 8 * L::kStages, accEmpty = accFull + 16, tmemSlot = accEmpty + 16;
+    const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kRaw; ++i)
+            dev::mbarInit(rawFull + 8 * i, TMA ? 1 : 3), dev::mbarInit(rawEmpty + 8 * i, 8); // warps of A and B
         for (int i = 0; i < L::kStages; ++i)
-            dev::mbarInit(full + 8 * i, 8), dev::mbarInit(empty + 8 * i, 1); // 4 warps of A, 4 of B
-        dev::mbarInit(done, 1);
+            dev::mbarInit(full + 8 * i, 8 * CG), dev::mbarInit(empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) // of a half of the columns
+            dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, 4 * CG);
         dev::fenceBarrierInit();
     }
-    if (warp == L::kMmaWarp) {
-        dev::tmemAlloc(tmemSlot, L::kTmemCols);
-        dev::tmemRelinquish();
-    }
+    if (warp == L::kMmaWarp)
+        tmemAllocGroup<CG>(tmemSlot, 512);
     dev::tcFenceBefore();
-    __syncthreads();
+    clusterSync<CG>();
     dev::tcFenceAfter();
-    const uint32_t tmem = dev::ldsU32(tmemSlot);
-    const uint32_t tiles = p.tilesN * p.tilesK;
-    const uint32_t tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-    const uint32_t n0 = tile % p.tilesN * 128, k0 = tile / p.tilesN * BK;
+    const uint32_t tmem = dev::ldsU32(tmemSlot), tmemA = tmem + 384;
+    const uint32_t unit = blockIdx.x / CG, tiles = p.tilesN * p.tilesK;
+    const uint32_t tile = unit % tiles, split = unit / tiles;
+    const uint32_t n0 = (tile % p.tilesN * CG + rank) * 128;
+    const uint32_t k0 = tile / p.tilesN * L::kBk, kMine = k0 + rank * L::kBCols;
     const uint64_t begin = uint64_t(split) * p.rowsPerSplit;
     const uint64_t end = min(uint64_t(p.rows), begin + p.rowsPerSplit);
     const uint32_t stages = uint32_t((end - begin + L::kRows - 1) / L::kRows);
+    // Flush e empties accumulator e % 3, which holds half e % 2: one every kFlush / 2 stages, and two
+    // after the last stage.
+    const uint32_t flushes = stages == 0 ? 0 : (stages - 1) / (L::kFlush / 2) + 2;
 
-    if (warp < L::kAWarps) {
-        // ---- A: stages warp / 4, + 2, ...; the warp's quarter of the 128 columns of dy ----
-        const uint32_t quarter = warp % 4, q4 = lane % 4;
-        const uint32_t col = n0 + 32 * quarter + 4 * (lane / 4);
-        const uint32_t left = col < p.n ? p.n - col : 0u;
-        const T* dy = static_cast<const T*>(p.dy);
-        constexpr int kJ = L::kRows / 16;
-        Quad<T> held[kJ][4]; // rows 16 j + 4 q4 + i
-        auto fetch = [&](uint32_t it) {
-            const uint64_t r0 = begin + uint64_t(it) * L::kRows + 4 * q4;
+    if (warp < L::kEpilogueWarps) {
+        registersUp<L::kRegsEpilogue>();
+        const uint32_t quarter = warp % 4, half = warp / 4;
+        float sum[128];
 #pragma unroll
-            for (int j = 0; j < kJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint64_t r = r0 + 16 * j + i;
-                    held[j][i] = loadQuad<T>(dy + r * p.dyStride + col, r < end ? left : 0u, p.vectorDy);
-                }
-        };
-        uint32_t it = warp / 4;
-        if (it < stages)
-            fetch(it);
-        for (; it < stages; it += 2) {
-            const uint32_t s = it % L::kStages, turn = it / L::kStages;
-            if (turn != 0 && !waitPhase(empty + 8 * s, (turn - 1) & 1))
-                break;
-            dev::tcFenceAfter();
-            const uint32_t to = tmem + BK + s * L::kACols + (quarter << 21);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t out[L::kP][4 * kJ];
-#pragma unroll
-                for (int j = 0; j < kJ; ++j)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) { // lane t / 4 + 8 (x / 2), column 8 j + 2 q4 + x % 2
-                        uint32_t part[L::kP];
-                        splitPair<T>(held[j][2 * (x % 2)], held[j][2 * (x % 2) + 1], 2 * half + x / 2, part);
-#pragma unroll
-                        for (int m = 0; m < L::kP; ++m)
-                            out[m][4 * j + x] = part[m];
-                    }
-#pragma unroll
-                for (int m = 0; m < L::kP; ++m)
-                    storeA<kJ>(to + m * (L::kRows / 2) + (half << 20), out[m]);
-            }
-            dev::tcWaitSt();
-            dev::tcFenceBefore();
-            __syncwarp();
-            if (lane == 0)
-                dev::mbarArrive(full + 8 * s);
-            if (it + 2 < stages)
-                fetch(it + 2);
-        }
-    } else if (warp < L::kAWarps + L::kBWarps) {
-        // ---- B: stages (warp - 8) / 4, + 2, ...; a quarter of the stage's rows per warp ----
-        constexpr int kLanes = BK / 8;              // lanes per row, 8 elements each
-        constexpr int kRowsAtOnce = 32 / kLanes;
-        constexpr int kWarpRows = L::kRows / 4;
-        constexpr int kLoads = kWarpRows / kRowsAtOnce;
-        constexpr int kKb = BK / 128;
-        const uint32_t w = warp % 4;
-        const uint32_t kk = lane % kLanes * 8, k = k0 + kk;
-        const uint32_t left = k < p.k ? p.k - k : 0u;
-        const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock;
-        const uint32_t scaleRow = lane / kKb, scaleCol = k0 / kBlock + lane % kKb;
-        uint2 held[kLoads];
-        uint32_t heldScale = 127;
-        auto fetch = [&](uint32_t it) {
-            const uint64_t r0 = begin + uint64_t(it) * L::kRows + w * kWarpRows;
-            heldScale = scaleRow < uint32_t(kWarpRows) && r0 + scaleRow < end && scaleCol < kBlocks
-                            ? __ldg(p.scales + (r0 + scaleRow) * kBlocks + scaleCol) : 127u;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint64_t r = r0 + i * kRowsAtOnce + lane / kLanes;
-                const uint8_t* src = p.q + r * p.qStride + k;
-                const uint32_t have = r < end ? left : 0u;
-                if (p.vectorQ && have >= 8) {
-                    held[i] = __ldg(reinterpret_cast<const uint2*>(src));
-                } else {
-                    uint32_t b[2] = {0, 0};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (uint32_t(e) < have)
-                            b[e / 4] |= uint32_t(__ldg(src + e)) << (8 * (e % 4));
-                    held[i] = make_uint2(b[0], b[1]);
-                }
-            }
-        };
-        uint32_t it = (warp - L::kAWarps) / 4;
-        if (it < stages)
-            fetch(it);
-        for (; it < stages; it += 2) {
-            const uint32_t s = it % L::kStages, turn = it / L::kStages;
-            if (turn != 0 && !waitPhase(empty + 8 * s, (turn - 1) & 1))
-                break;
-            // Column group kk / 64: kRows rows of 128 bytes; 16-byte pieces swizzled by the row.
-            const uint32_t to = base + s * L::kBBytes + kk / 64 * (L::kRows * 128);
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint32_t row = i * kRowsAtOnce + lane / kLanes;
-                const __nv_bfloat162 scale =
-                    scalePair(__shfl_sync(0xFFFFFFFFu, heldScale, row * kKb + kk / 128));
-                uint32_t o[4];
-                int8ToBf16(held[i].x, scale, o[0], o[1]);
-                int8ToBf16(held[i].y, scale, o[2], o[3]);
-                const uint32_t r = w * kWarpRows + row;
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                             ::"r"(to + r * 128 + (((kk / 8) ^ r) & 7) * 16), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
-                             : "memory");
-            }
-            dev::fenceProxyAsyncShared();
-            __syncwarp();
-            if (lane == 0)
-                dev::mbarArrive(full + 8 * s);
-            if (it + 2 < stages)
-                fetch(it + 2);
-        }
-    } else if (lane == 0) {
-        // ---- MMA issue ----
+        for (int i = 0; i < 128; ++i)
+            sum[i] = 0.0f;
         bool ok = true;
-        for (uint32_t it = 0; it < stages; ++it) {
-            const uint32_t s = it % L::kStages;
-            if (!waitPhase(full + 8 * s, (it / L::kStages) & 1)) {
+        for (uint32_t e = half; e < flushes; e += 2) {
+            const uint32_t acc = e % 3;
+            if (!waitCluster<CG>(accFull + 8 * half, (e / 2) & 1)) {
                 ok = false;
                 break;
             }
             dev::tcFenceAfter();
-            const uint32_t a = tmem + BK + s * L::kACols;
-            const uint64_t b = swizzledDesc(base + s * L::kBBytes, L::kRows * 128, 1024);
 #pragma unroll
-            for (int j = 0; j < L::kRows / 16; ++j)
-#pragma unroll
-                for (int m = 0; m < L::kP; ++m)
-                    mmaBf16Ts(tmem, a + m * (L::kRows / 2) + 8 * j, b + 128 * j, bf16Idesc(BK), (it | j | m) != 0);
-            dev::tcCommit(empty + 8 * s);
-        }
-        if (ok)
-            dev::tcCommit(done);
-    }
-    __syncwarp();
-    // ---- dW or a partial tile: eight warps, half of the columns each ----
-    if (warp < 8 && (stages == 0 || waitPhase(done, 0))) {
-        dev::tcFenceAfter();
-        const uint32_t quarter = warp % 4, half = warp / 4;
-        const uint32_t row = n0 + 32 * quarter + laneColumn(lane);
-#pragma unroll
-        for (int c = 0; c < BK / 2; c += 32) {
-            const uint32_t col = half * (BK / 2) + c;
-            uint32_t r[32];
-            if (stages != 0) {
-                tcLoad32x32bx32(tmem + col + (quarter << 21), r);
+            for (int c = 0; c < 128; c += 16) {
+                uint32_t r[16];
+                dev::tcLoad32x32bx16(tmem + acc * 128 + c + (quarter << 21), r);
                 dev::tcWaitLd();
-            } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    r[i] = 0u;
+                for (int i = 0; i < 16; ++i)
+                    sum[c + i] += __uint_as_float(r[i]);
             }
-            if (p.partials != nullptr) {
-                float4* out = reinterpret_cast<float4*>(p.partials) + uint64_t(blockIdx.x) * (128 * BK / 4) +
-                              (col / 4) * 128 + 32 * quarter + lane;
+            dev::tcFenceBefore();
+            __syncwarp();
+            if (lane == 0)
+                arriveLeader<CG>(accEmpty + 8 * half);
+        }
+        const uint32_t row = n0 + 32 * quarter + laneColumn(lane);
+        if (ok && p.partials != nullptr) {
+            float4* out = reinterpret_cast<float4*>(p.partials) + uint64_t(blockIdx.x) * (128 * L::kBk / 4) + half * 32 * 128 +
+                          32 * quarter + lane;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    out[128 * i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
-                                               __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-            } else if (row < p.n) {
-                float* out = p.dw + row * p.dwStride + k0 + col;
-                if (p.dwAlign != 0 && k0 + col + 32 <= p.k) {
+            for (int i = 0; i < 32; ++i)
+                out[128 * i] = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+        } else if (ok && row < p.n) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
-                                               __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-                        float4* o = reinterpret_cast<float4*>(out) + i;
-                        if (p.accumulate) {
-                            const float4 was = *o;
-                            v = make_float4(v.x + was.x, v.y + was.y, v.z + was.z, v.w + was.w);
-                        }
-                        *o = v;
+            for (int i = 0; i < 128; i += 4) {
+                const uint32_t col = k0 + columnOf<CG>(half, i);
+                float* out = p.dw + row * p.dwStride + col;
+                if (p.dwVector && col + 4 <= p.k) {
+                    float4 v = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+                    if (p.accumulate) {
+                        const float4 was = *reinterpret_cast<const float4*>(out);
+                        v = make_float4(v.x + was.x, v.y + was.y, v.z + was.z, v.w + was.w);
                     }
+                    *reinterpret_cast<float4*>(out) = v;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (k0 + col + i < p.k)
-                            out[i] = __uint_as_float(r[i]) + (p.accumulate ? out[i] : 0.0f);
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < p.k)
+                            out[j] = sum[i + j] + (p.accumulate ? out[j] : 0.0f);
                 }
             }
         }
+    } else if (warp < L::kBWarp) {
+        registersDown<L::kRegsConvert>();
+        // ---- A: the warp's quarter of the 128 columns of dy ----
+        const uint32_t quarter = warp % 4, q4 = lane % 4;
+        const uint32_t byte = (32 * quarter + 4 * (lane / 4)) * sizeof(T); // of the thread's columns in a raw row
+        const uint32_t from = base + L::kRawOff + byte / 128 * L::kBox, within = byte % 128;
+        uint32_t raw = 0, rawPhase = 0, s = 0, phase = 1; // a stage's first turn does not wait
+        for (uint32_t it = 0; it < stages; ++it) {
+            if (!waitPhase(rawFull + 8 * raw, rawPhase) || !waitCluster<CG>(empty + 8 * s, phase))
+                break;
+            dev::tcFenceAfter();
+            const uint32_t src = from + raw * L::kRawBytes;
+            const uint32_t to = tmemA + s * L::kACols + (quarter << 21);
+#pragma unroll
+            for (int j = 0; j < L::kRows / 16; ++j) {
+                Quad<T> q[4]; // operand rows 16 j + 4 q4 + i
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t r = 16 * j + 8 * (i / 2) + 2 * q4 + i % 2;
+                    q[i] = loadQuad<T>(src + r * 128 + (within ^ ((r & 7) << 4)));
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t out[4][L::kP];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) // lane t / 4 + 8 (x / 2), column 8 j + 2 q4 + x % 2
+                        splitPair<T>(q[2 * (x % 2)], q[2 * (x % 2) + 1], 2 * half + x / 2, out[x]);
+#pragma unroll
+                    for (int m = 0; m < L::kP; ++m)
+                        tcStore16x256b(to + m * (L::kRows / 2) + 8 * j + (half << 20), out[0][m], out[1][m], out[2][m],
+                                       out[3][m]);
+                }
+            }
+            dev::tcWaitSt();
+            dev::tcFenceBefore();
+            __syncwarp();
+            if (lane == 0) {
+                dev::mbarArrive(rawEmpty + 8 * raw);
+                arriveLeader<CG>(full + 8 * s);
+            }
+            if (++raw == L::kRaw)
+                raw = 0, rawPhase ^= 1;
+            if (++s == L::kStages)
+                s = 0, phase ^= 1;
+        }
+    } else if (warp < L::kLoadWarp) {
+        registersDown<L::kRegsConvert>();
+        // ---- B: a quarter of the stage's rows per warp, 16 lanes of 8 columns per row and box ----
+        constexpr uint32_t kWarpRows = L::kRows / 4;
+        const uint32_t first = (warp - L::kBWarp) * kWarpRows;
+        const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock;
+        const uint32_t sRow = lane % kWarpRows, sBox = lane / kWarpRows;
+        const uint32_t sCol = kMine / kBlock + sBox;
+        const bool sMine = sBox < uint32_t(L::kBBoxes) && sCol < kBlocks;
+        auto scaleOf = [&](uint32_t it) {
+            const uint64_t r = begin + uint64_t(it) * L::kRows + first + sRow;
+            return sMine && it < stages && r < end ? uint32_t(__ldg(p.scales + r * kBlocks + sCol)) : 127u;
+        };
+        uint32_t scale0 = scaleOf(0), scale1 = scaleOf(1); // two stages ahead
+        uint32_t raw = 0, rawPhase = 0, s = 0, phase = 1;
+        for (uint32_t it = 0; it < stages; ++it) {
+            const uint32_t scales = scale0;
+            scale0 = scale1;
+            scale1 = scaleOf(it + 2);
+            if (!waitPhase(rawFull + 8 * raw, rawPhase) || !waitCluster<CG>(empty + 8 * s, phase))
+                break;
+            const uint32_t src = base + L::kRawOff + raw * L::kRawBytes + L::kABoxes * L::kBox;
+            const uint32_t to = base + s * L::kBBytes;
+#pragma unroll
+            for (int box = 0; box < L::kBBoxes; ++box)
+#pragma unroll
+                for (uint32_t i = 0; i < kWarpRows; i += 2) {
+                    const uint32_t local = i + lane / 16, r = first + local, c = lane % 16;
+                    const uint2 w = dev::ldsV2(src + box * L::kBox + r * 128 + 8 * c);
+                    const __nv_bfloat162 scale =
+                        scalePair(__shfl_sync(0xFFFFFFFFu, scales, local + box * kWarpRows));
+                    uint32_t o[4];
+                    int8ToBf16(w.x, scale, o[0], o[1]);
+                    int8ToBf16(w.y, scale, o[2], o[3]);
+                    const uint32_t k = operandRow(r);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(to + (2 * box + c / 8) * L::kBox + k * 128 + ((c ^ k) & 7) * 16), "r"(o[0]),
+                                 "r"(o[1]), "r"(o[2]), "r"(o[3])
+                                 : "memory");
+                }
+            dev::fenceProxyAsyncShared();
+            __syncwarp();
+            if (lane == 0) {
+                dev::mbarArrive(rawEmpty + 8 * raw);
+                arriveLeader<CG>(full + 8 * s);
+            }
+            if (++raw == L::kRaw)
+                raw = 0, rawPhase ^= 1;
+            if (++s == L::kStages)
+                s = 0, phase ^= 1;
+        }
+    } else {
+        registersDown<L::kRegsIssue>();
+        if (warp == L::kMmaWarp) {
+            if (lane == 0 && rank == 0) {
+                // ---- MMA issue ----
+                uint32_t s = 0, phase = 0, flushed = 0;
+                uint32_t acc[2] = {0, 1};
+                bool fresh[2] = {true, true}, ok = true;
+                auto flush = [&](uint32_t h) { // the half goes on in the accumulator that was flushed before
+                    commitCluster<CG>(accFull + 8 * h);
+                    acc[h] = (flushed + 2) % 3;
+                    fresh[h] = true;
+                    ++flushed;
+                };
+                for (uint32_t it = 0; it < stages && ok; ++it) {
+                    if (!waitCluster<CG>(full + 8 * s, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    dev::tcFenceAfter();
+                    const uint32_t a = tmemA + s * L::kACols;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        // The accumulator of a fresh half was emptied by the flush before the half's own
+                        // last one, which the epilogue must have read out.
+                        if (fresh[h] && flushed >= 2) {
+                            const uint32_t before = flushed - 2;
+                            if (!waitCluster<CG>(accEmpty + 8 * (before % 2), (before / 2) & 1)) {
+                                ok = false;
+                                break;
+                            }
+                            dev::tcFenceAfter();
+                        }
+                        const uint32_t b = base + s * L::kBBytes + h * (2 / CG) * L::kBox;
+                        const uint64_t desc = swizzledDesc(b, L::kBox, 1024);
+#pragma unroll
+                        for (int j = 0; j < L::kRows / 16; ++j)
+#pragma unroll
+                            for (int m = 0; m < L::kP; ++m) {
+                                mmaBf16Ts<CG>(tmem + acc[h] * 128, a + m * (L::kRows / 2) + 8 * j, desc + 128 * j,
+                                              bf16Idesc(128 * CG, 128), !(fresh[h] && j == 0 && m == 0));
+                            }
+                        fresh[h] = false;
+                    }
+                    if (!ok)
+                        break;
+                    commitCluster<CG>(empty + 8 * s);
+                    if ((it + 1) % (L::kFlush / 2) == 0 && it + 1 < stages)
+                        flush(flushed % 2);
+                    if (++s == L::kStages)
+                        s = 0, phase ^= 1;
+                }
+                if (ok && stages != 0) {
+                    flush(flushed % 2);
+                    flush(flushed % 2);
+                }
+            }
+        } else if constexpr (TMA) {
+            if (warp == L::kLoadWarp && lane == 0) {
+                tmaPrefetchMap(&mapDy);
+                tmaPrefetchMap(&mapQ);
+                uint32_t raw = 0, phase = 1, it = 0;
+                bool ok = true;
+                for (; it < stages; ++it) {
+                    if (!waitPhase(rawEmpty + 8 * raw, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t to = base + L::kRawOff + raw * L::kRawBytes, bar = rawFull + 8 * raw;
+                    const uint32_t r = uint32_t(begin) + it * L::kRows;
+                    dev::mbarArriveExpectTx(bar, L::kRawBytes);
+#pragma unroll
+                    for (int i = 0; i < L::kABoxes; ++i)
+                        tmaLoad2d(to + i * L::kBox, &mapDy, n0 + i * (128 / uint32_t(sizeof(T))), r, bar);
+#pragma unroll
+                    for (int i = 0; i < L::kBBoxes; ++i)
+                        tmaLoad2d(to + (L::kABoxes + i) * L::kBox, &mapQ, kMine + 128 * i, r, bar);
+                    if (++raw == L::kRaw)
+                        raw = 0, phase ^= 1;
+                }
+                // After a wait that ran out, no copy may still be on its way when the CTA exits.
+                if (!ok)
+                    for (uint32_t i = it < L::kRaw ? 0 : it - L::kRaw; i < it; ++i)
+                        waitPhase(rawFull + 8 * (i % L::kRaw), (i / L::kRaw) & 1);
+            }
+        } else {
+            // ---- raw stages element by element, for rows that do not start on 16 bytes: three warps ----
+            uint32_t raw = 0, phase = 1;
+            for (uint32_t it = 0; it < stages; ++it) {
+                if (!waitPhase(rawEmpty + 8 * raw, phase))
+                    break;
+                const uint32_t to = base + L::kRawOff + raw * L::kRawBytes;
+                for (uint32_t r = warp - L::kLoadWarp; r < uint32_t(L::kRows); r += 3) {
+                    const uint64_t row = begin + uint64_t(it) * L::kRows + r;
+                    const bool in = row < end;
+                    const T* dy = static_cast<const T*>(p.dy) + row * p.dyStride + n0;
+                    for (uint32_t c = lane; c < 128; c += 32) {
+                        const uint32_t byte = c * sizeof(T), at = to + byte / 128 * L::kBox + r * 128 + ((byte % 128) ^ ((r & 7) << 4));
+                        const bool valid = in && n0 + c < p.n;
+                        if constexpr (sizeof(T) == 4) {
+                            const uint32_t v = valid ? __ldg(reinterpret_cast<const uint32_t*>(dy) + c) : 0u;
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+                        } else {
+                            const unsigned short v = valid ? __ldg(reinterpret_cast<const unsigned short*>(dy) + c) : 0;
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+                        }
+                    }
+                    const uint8_t* q = p.q + row * p.qStride + kMine;
+                    for (uint32_t c = lane; c < uint32_t(L::kBCols); c += 32) {
+                        const uint32_t at = to + (L::kABoxes + c / 128) * L::kBox + r * 128 + c % 128;
+                        const unsigned short v = in && kMine + c < p.k ? __ldg(q + c) : 0;
+                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+                    }
+                }
+                __syncwarp();
+                if (lane == 0)
+                    dev::mbarArrive(rawFull + 8 * raw);
+                if (++raw == L::kRaw)
+                    raw = 0, phase ^= 1;
+            }
+        }
     }
+    __syncwarp();
     dev::tcFenceBefore();
-    __syncthreads();
+    clusterSync<CG>(); // no CTA of a pair leaves while the other may still arrive on its barriers
     dev::tcFenceAfter();
     if (warp == L::kMmaWarp)
-        dev::tmemDealloc(tmem, L::kTmemCols);
+        tmemDeallocGroup<CG>(tmem, 512);
 }
 
 // dW (+)= the partial tiles, added in the order of their row ranges within eight interleaved sums
-// that are then added in order: the result does not depend on timing. 32 float4 columns of a
-// partial tile per CTA, eight threads each.
-__global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t splits, uint32_t bk) {
+// that are then added in order: the result does not depend on timing. 32 float4 columns of a CTA's
+// partial tile per block, eight threads each.
+template <int CG>
+__global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t splits) {
     __shared__ float4 sums[8][32];
-    const uint32_t perTile = 128 * bk / 4;
+    constexpr uint32_t kPerCta = 128 * 256 / 4;
     const uint64_t item = uint64_t(blockIdx.x) * 32 + threadIdx.x % 32;
-    const uint32_t tile = uint32_t(item / perTile), within = uint32_t(item % perTile);
+    const uint32_t cta = uint32_t(item / kPerCta), within = uint32_t(item % kPerCta);
     const uint32_t part = threadIdx.x / 32;
-    const uint64_t step = uint64_t(p.tilesN) * p.tilesK * perTile;
+    const uint64_t step = uint64_t(p.tilesN) * p.tilesK * CG * kPerCta;
     const float4* in = reinterpret_cast<const float4*>(p.partials) + item;
     float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll 4
@@ -415,8 +530,9 @@ __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t sp
         const float4 v = sums[i][threadIdx.x];
         sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
     }
-    const uint32_t l = within % 128, row = tile % p.tilesN * 128 + l / 32 * 32 + laneColumn(l % 32);
-    const uint32_t col = tile / p.tilesN * bk + within / 128 * 4;
+    const uint32_t l = within % 128, c = within / 128 * 4, tile = cta / CG;
+    const uint32_t row = (tile % p.tilesN * CG + cta % CG) * 128 + l / 32 * 32 + laneColumn(l % 32);
+    const uint32_t col = tile / p.tilesN * 256 + columnOf<CG>(c / 128, c % 128);
     if (row >= p.n || col >= p.k)
         return;
     float* out = p.dw + row * p.dwStride + col;
@@ -432,23 +548,24 @@ __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t sp
 // ranges is the cheapest by an estimate for 148 SMs: waves of CTAs, each row of a range at the MMA
 // rate and each CTA with a fixed start and end, against the partial tiles' traffic.
 struct Plan {
-    uint32_t bk, tilesN, tilesK, splits, rowsPerSplit;
+    int cg;
+    uint32_t tilesN, tilesK, splits, rowsPerSplit;
 };
 Plan planOf(uint32_t rows, uint32_t n, uint32_t k) {
-    constexpr double kSms = 148, kFixedUs = 4, kSumUs = 4;
+    constexpr double kSms = 148, kFixedUs = 5, kSumUs = 4;
     Plan p{};
-    p.bk = k <= 128 ? 128 : 256;
-    p.tilesN = ceilDiv(n, 128u);
-    p.tilesK = ceilDiv(k, p.bk);
+    p.cg = n <= 128 ? 1 : 2;
+    p.tilesN = ceilDiv(n, 128u * p.cg);
+    p.tilesK = ceilDiv(k, 256u);
     const double tiles = double(p.tilesN) * p.tilesK;
     const uint32_t steps = std::max(1u, ceilDiv(rows, 64u));
-    const double stepUs = 0.35 * p.bk / 256, tileUs = 128.0 * p.bk * 4 * 2 / 5e6; // a partial tile out and in
+    const double stepUs = 0.4, tileUs = p.cg * 128.0 * 256 * 4 * 2 / 5e6; // 64 rows; a partial tile out and in
     double best = 0;
     for (uint32_t splits = 1; splits <= steps && splits <= 296; ++splits) {
         const uint32_t per = ceilDiv(steps, splits);
         if (ceilDiv(steps, per) != splits)
             continue;
-        const double waves = std::ceil(tiles * splits / kSms);
+        const double waves = std::ceil(tiles * splits * p.cg / kSms);
         const double us = waves * (per * stepUs + kFixedUs) + (splits > 1 ? kSumUs + splits * tiles * tileUs : 0);
         if (splits == 1 || us < best) {
             best = us;
@@ -459,23 +576,54 @@ Plan planOf(uint32_t rows, uint32_t n, uint32_t k) {
     return p;
 }
 uint64_t workspaceBytes(const Plan& p) {
-    return p.splits > 1 ? uint64_t(p.splits) * p.tilesN * p.tilesK * 128 * p.bk * 4 : 0;
+    return p.splits > 1 ? uint64_t(p.splits) * p.tilesN * p.tilesK * p.cg * 128 * 256 * 4 : 0;
 }
 
-template <typename T, int BK> void launchTiles(const GradArgs& g, const Plan& p, cudaStream_t stream) {
-    using L = GradTile<T, BK>;
-    const uint64_t grid = uint64_t(p.tilesN) * p.tilesK * p.splits;
+template <typename T, int CG, bool TMA>
+void launchTiles(const GradArgs& g, const Plan& p, int type, cudaStream_t stream) {
+    using L = GradTile<T, CG>;
+    constexpr auto kernel = gradTiles<T, CG, TMA>;
+    // The kernel shares its launch's registers out anew and would wait for ever for ones that it
+    // did not get.
+    static const int regs = [] {
+        cudaFuncAttributes attr{};
+        checkCudaCall(cudaFuncGetAttributes(&attr, gradTiles<T, CG, TMA>));
+        return attr.numRegs;
+    }();
+    if (regs != L::kRegs)
+        throw CudaError("weight_grad_int8 was built with an unexpected register count");
+    const uint64_t grid = uint64_t(p.tilesN) * p.tilesK * p.splits * CG;
     require(grid <= 0x7FFFFFFFull, "too many output tiles for one call");
-    allowSharedMemory<gradTiles<T, BK>>(L::kBytes);
-    gradTiles<T, BK><<<uint32_t(grid), L::kThreads, L::kBytes, stream>>>(g);
-    checkCudaCall(cudaGetLastError());
+    CUtensorMap mapDy{}, mapQ{};
+    if constexpr (TMA) {
+        const auto t = type == TCC_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == TCC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        mapDy = tensorMap2d(g.dy, t, sizeof(T), g.rows, g.n, g.dyStride, L::kRows, 128 / sizeof(T));
+        mapQ = tensorMap2d(g.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.rows, g.k, g.qStride, L::kRows, 128,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+    allowSharedMemory<gradTiles<T, CG, TMA>>(L::kBytes);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(uint32_t(grid));
+    config.blockDim = dim3(L::kThreads);
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    checkCudaCall(cudaLaunchKernelEx(&config, kernel, mapDy, mapQ, g));
     if (p.splits > 1) {
-        sumPartials<<<p.tilesN * p.tilesK * (128 * BK / 4 / 32), 256, 0, stream>>>(g, p.splits, BK);
+        sumPartials<CG><<<p.tilesN * p.tilesK * CG * (128 * 256 / 4 / 32), 256, 0, stream>>>(g, p.splits);
         checkCudaCall(cudaGetLastError());
     }
 }
-template <typename T> void launchGrad(const GradArgs& g, const Plan& p, cudaStream_t stream) {
-    p.bk == 128 ? launchTiles<T, 128>(g, p, stream) : launchTiles<T, 256>(g, p, stream);
+template <typename T> void launchGrad(const GradArgs& g, const Plan& p, int type, bool tma, cudaStream_t stream) {
+    if (p.cg == 1)
+        tma ? launchTiles<T, 1, true>(g, p, type, stream) : launchTiles<T, 1, false>(g, p, type, stream);
+    else
+        tma ? launchTiles<T, 2, true>(g, p, type, stream) : launchTiles<T, 2, false>(g, p, type, stream);
 }
 
 } // namespace
@@ -524,15 +672,15 @@ int tcc_weight_grad_int8(const void* grad_y, int type, uint64_t grad_y_stride, c
         g.rows = rows, g.n = n, g.k = k;
         g.tilesN = p.tilesN, g.tilesK = p.tilesK, g.rowsPerSplit = p.rowsPerSplit;
         g.accumulate = accumulate != 0;
-        g.vectorDy = rowsAlignedTo(grad_y, grad_y_stride * typeBytes(type), 4 * typeBytes(type));
-        g.vectorQ = rowsAlignedTo(q, q_stride, 8);
-        const uint64_t rowBytes = grad_w_stride * 4;
-        g.dwAlign = rowsAlignedTo(grad_w, rowBytes, 16) ? 16 : 0;
+        g.dwVector = rowsAlignedTo(grad_w, grad_w_stride * 4, 16);
+        const bool tma = rows != 0 && rowsAlignedTo(grad_y, grad_y_stride * typeBytes(type), 16) &&
+                         rowsAlignedTo(q, q_stride, 16) && grad_y_stride < (1ull << 38) && q_stride < (1ull << 40) &&
+                         std::max({rows, n, k}) <= 0x7FFFFF00u; // coordinates of a copy are signed
         auto s = reinterpret_cast<cudaStream_t>(stream);
         switch (type) {
-        case TCC_F32: launchGrad<float>(g, p, s); break;
-        case TCC_BF16: launchGrad<__nv_bfloat16>(g, p, s); break;
-        default: launchGrad<__half>(g, p, s); break;
+        case TCC_F32: launchGrad<float>(g, p, type, tma, s); break;
+        case TCC_BF16: launchGrad<__nv_bfloat16>(g, p, type, tma, s); break;
+        default: launchGrad<__half>(g, p, type, tma, s); break;
         }
     });
 }
