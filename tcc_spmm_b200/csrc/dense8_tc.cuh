@@ -59,19 +59,42 @@ __device__ __forceinline__ uint64_t slabDesc(uint32_t addr) {
 }
 
 // 32 rows x 16 bytes from shared memory to 4 tensor-memory columns, repeated in the four lane
-// quarters: row i's word c lands in lanes i, i + 32, i + 64 and i + 96 of column c.
-__device__ __forceinline__ void tcCopyScales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// quarters: row i's word c lands in lanes i, i + 32, i + 64 and i + 96 of column c. In every CTA of a
+// pair, from its own shared memory.
+template <int CG> __device__ __forceinline__ void tcCopyScales(uint32_t elected, uint32_t taddr, uint64_t desc) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+                     "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+                     "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
+                     : "memory");
 }
 
+// The MMA issuing warps run in uniform control flow, so that the operands stay in uniform registers
+// (an MMA issued inside a one-lane branch moves each operand there first, which took longer than the
+// MMA itself), and one elected lane issues.
+__device__ __forceinline__ uint32_t electLane() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
 // D(tmem) (+)= A x B from shared memory, 8-bit floats with E8M0 scales in tensor memory (one per 32
-// elements of k).
-__device__ __forceinline__ void mmaScaled8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scaleA,
-                                           uint32_t scaleB, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate)
-                 : "memory");
+// elements of k), by the lane with `elected`.
+template <int CG>
+__device__ __forceinline__ void mmaScaled8(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t scaleA, uint32_t scaleB, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+                     "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate), "r"(elected)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\t"
+                     "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate), "r"(elected)
+                     : "memory");
 }
 
 // Warp load of 32 TMEM lanes x 32 columns: thread t reads lane t, r[j] = column j.
@@ -139,13 +162,17 @@ template <int CG> __device__ __forceinline__ bool waitCluster(uint32_t bar, uint
     }
 }
 // One arrival on the barrier at this address in every CTA of the cluster, once the tcgen05
-// operations that this thread issued are done.
-template <int CG> __device__ __forceinline__ void commitCluster(uint32_t bar) {
+// operations that the elected lane issued are done.
+template <int CG> __device__ __forceinline__ void commitCluster(uint32_t elected, uint32_t bar) {
     if constexpr (CG == 1)
-        dev::tcCommit(bar);
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+                     "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                     ::"r"(bar), "r"(elected)
+                     : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                     ::"r"(bar), "h"(static_cast<unsigned short>(3))
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+                     "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}"
+                     ::"r"(bar), "r"(elected), "h"(static_cast<unsigned short>(3))
                      : "memory");
 }
 template <int CG> __device__ __forceinline__ void tmemAllocGroup(uint32_t dst, uint32_t cols) {

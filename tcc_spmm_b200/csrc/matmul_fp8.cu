@@ -300,53 +300,61 @@ __global__ void __launch_bounds__(Tile<BN, KN>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp == L::kMmaWarp) {
-        if (lane == 0) {
-            uint32_t it = 0, group = 0, seq = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++seq) {
-                const uint32_t acc = seq % L::kAcc, accTurn = seq / L::kAcc;
-                if (accTurn != 0 && !waitPhase(accEmpty + 8 * acc, (accTurn - 1) & 1))
-                    break;
-                dev::tcFenceAfter();
-                const uint32_t d = tmem + acc * BN;
-                for (uint32_t kb = 0; kb < kBlocks; ++kb, ++it) {
-                    const uint32_t slot = group % L::kSlots;
-                    const uint32_t sa = scaleTmem + slot * L::kScaleCols, sb = sa + 4;
-                    if (kb % 4 == 0) {
-                        if (!waitPhase(scaleFull + 8 * slot, (group / L::kSlots) & 1)) {
-                            ok = false;
-                            break;
-                        }
-                        dev::tcFenceAfter();
-                        const uint32_t slab = base + L::kScaleOff + slot * L::kSlabs * 512;
-#pragma unroll
-                        for (int i = 0; i < L::kSlabs; ++i)
-                            tcCopyScales(sa + 4 * i, slabDesc(slab + 512 * i));
-                    }
-                    const uint32_t s = it % L::kStages;
-                    if (!waitPhase(full + 8 * s, (it / L::kStages) & 1)) {
+        // The whole warp in uniform control flow; one elected lane issues.
+        const uint32_t elected = electLane();
+        uint32_t stage = 0, phase = 0, slot = 0, slotPhase = 0, acc = 0, accPhase = 1; // an accumulator's first turn does not wait
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            if (!waitPhase(accEmpty + 8 * acc, accPhase))
+                break;
+            dev::tcFenceAfter();
+            const uint32_t d = tmem + acc * BN;
+            for (uint32_t kb = 0; kb < kBlocks; ++kb) {
+                const uint32_t sa = scaleTmem + slot * L::kScaleCols, sb = sa + 4, byte = kb & 3;
+                if (byte == 0) {
+                    if (!waitPhase(scaleFull + 8 * slot, slotPhase)) {
                         ok = false;
                         break;
                     }
                     dev::tcFenceAfter();
-                    const uint32_t a = base + s * L::kStageBytes, b = a + L::kABytes;
-                    const uint64_t descA = swizzledDesc(a, 16, 1024);
-                    const uint64_t descB = KN ? swizzledDesc(b, 16384, 1024) : swizzledDesc(b, 16, 1024);
-                    const uint32_t idesc = p.idesc | ((kb % 4) << 29) | ((kb % 4) << 4);
-                    const uint32_t steps = min(4u, (p.k - kb * kBlock + 31) / 32);
-                    for (uint32_t j = 0; j < steps; ++j)
-                        mmaScaled8(d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
-                    dev::tcCommit(empty + 8 * s);
-                    if (kb % 4 == 3 || kb + 1 == kBlocks) {
-                        dev::tcCommit(scaleEmpty + 8 * slot);
-                        ++group;
-                    }
+                    const uint32_t slab = base + L::kScaleOff + slot * L::kSlabs * 512;
+#pragma unroll
+                    for (int i = 0; i < L::kSlabs; ++i)
+                        tcCopyScales<1>(elected, sa + 4 * i, slabDesc(slab + 512 * i));
                 }
-                if (ok)
-                    dev::tcCommit(accFull + 8 * acc);
+                if (!waitPhase(full + 8 * stage, phase)) {
+                    ok = false;
+                    break;
+                }
+                dev::tcFenceAfter();
+                const uint32_t a = base + stage * L::kStageBytes, b = a + L::kABytes;
+                const uint64_t descA = swizzledDesc(a, 16, 1024);
+                const uint64_t descB = KN ? swizzledDesc(b, 16384, 1024) : swizzledDesc(b, 16, 1024);
+                const uint32_t idesc = p.idesc | (byte << 29) | (byte << 4);
+                if (p.k - kb * kBlock >= kBlock) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mmaScaled8<1>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb,
+                                      j != 0 ? 1u : uint32_t(kb != 0));
+                } else { // the last block ends inside
+                    const uint32_t steps = (p.k - kb * kBlock + 31) / 32;
+                    for (uint32_t j = 0; j < steps; ++j)
+                        mmaScaled8<1>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
+                }
+                commitCluster<1>(elected, empty + 8 * stage);
+                if (++stage == L::kStages)
+                    stage = 0, phase ^= 1;
+                if (byte == 3 || kb + 1 == kBlocks) {
+                    commitCluster<1>(elected, scaleEmpty + 8 * slot);
+                    if (++slot == L::kSlots)
+                        slot = 0, slotPhase ^= 1;
+                }
             }
+            if (ok)
+                commitCluster<1>(elected, accFull + 8 * acc);
+            if (++acc == L::kAcc)
+                acc = 0, accPhase ^= 1;
         }
-        __syncwarp();
     } else if (warp == L::kScaleWarp) {
         // Lane i holds rows i, i + 32, i + 64 and i + 96 of a slab, 16 bytes in shared memory.
         constexpr int kWords = 4 * L::kSlabs;

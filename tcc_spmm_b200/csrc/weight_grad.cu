@@ -11,16 +11,16 @@
 // of q^, which halves the conversions and the shared-memory reads of an SM. CG = 1 where dW has at
 // most 128 rows.
 //
-// Raw rows arrive by TMA in a ring of stages. Four warps turn dy into operand A in tensor memory: a
-// thread takes four neighbouring columns of a row at a time and pairs rows with byte permutes. Four
+// Raw rows arrive by TMA in a ring of stages. Eight warps turn dy into operand A in tensor memory: a
+// thread takes four neighbouring columns of a row at a time and pairs rows with byte permutes. Eight
 // warps turn q into operand B in shared memory, row-major as it comes (MN-major, 128-byte swizzle).
 // One thread issues the MMAs.
 //
 // The tensor core cuts off what an addition shifts out below the accumulator's last bit, about
 // 1.5e-8 of the sum for every MMA (measured; 2.1e-5 after 1300), so the accumulator is emptied every
-// kFlush MMAs into fp32 registers, which round to nearest. The two halves of the 256 columns take
-// turns, half a period apart, over three accumulators of 128 columns: the MMAs go on in the third
-// while eight warps read one out.
+// 48 to 60 MMAs into fp32 registers, which round to nearest. The two halves of the 256 columns are
+// issued in turns of kTurn stages, half a turn apart: eight warps read one half out while the other's
+// turn runs.
 #include "dense8.cuh"
 #include "dense8_tc.cuh"
 
@@ -46,34 +46,45 @@ struct GradArgs {
     bool dwVector; // rows of dw start on 16 bytes
 };
 
+template <uint32_t V> struct Const { static constexpr uint32_t value = V; };
+
 template <typename T> constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
 template <> constexpr int kParts<__half> = 2;
 
 template <typename T, int CG> struct GradTile {
     static constexpr int kP = kParts<T>;
-    static constexpr int kRows = kP == 3 ? 32 : 64;    // rows per stage
+    static constexpr int kRows = kP == 3 || CG == 1 ? 32 : 64; // rows per stage
     static constexpr int kBk = 256, kBCols = kBk / CG; // columns of dW: of the cluster, of q in this CTA
-    static constexpr int kRaw = CG == 1 && kP < 3 ? 3 : 6, kStages = kP == 1 ? 3 : 2;
+    // Raw and operand stages: an operand stage takes about a microsecond from its conversion over the
+    // MMAs' completion to its next use, so that much has to be in flight.
+    static constexpr int kRaw = kP == 3 ? (CG == 1 ? 6 : 8) : CG == 1 || kP == 2 ? 6 : 4;
+    static constexpr int kStages = kP == 3 || (kP == 2 && CG == 2) ? 4 : 6;
+    // Two sets of producer warps take alternate stages. In an even ring a place always belongs to the
+    // same set; in an odd one a set could run two of the place's phases ahead of the other, where a
+    // barrier's parity no longer tells done from not yet begun.
+    static_assert(kRaw % 2 == 0 && kStages % 2 == 0, "even rings");
     static constexpr int kABoxes = int(sizeof(T)), kBBoxes = kBCols / 128; // of 128 bytes x kRows
     static constexpr int kBox = kRows * 128;
     static constexpr int kRawBytes = (kABoxes + kBBoxes) * kBox;
     static constexpr int kBBytes = kRows * kBCols * 2;
     static constexpr int kACols = kP * kRows / 2;       // tensor-memory columns of a stage of A
     static constexpr int kSteps = kP * kRows / 16;      // MMAs per stage and accumulator
-    static constexpr int kFlush = 60 / kSteps / 2 * 2;  // stages between two flushes of a half (even)
+    static constexpr uint32_t kTurn = kStages >= 6 ? 4 : 2;               // stages of a half in one go
+    static constexpr uint32_t kFlush = 60 / kSteps / kTurn * kTurn;        // stages between two flushes of a half
     static constexpr int kRawOff = kStages * kBBytes;
-    static constexpr int kBarOff = kRawOff + kRaw * kRawBytes;
-    // rawFull, rawEmpty [kRaw]; full, empty [kStages]; accFull, accEmpty [2]; TMEM address
-    static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 2 * kStages + 4) + 16 + 1024;
-    static constexpr int kCols = 3 * 128 + kStages * kACols;
-    static constexpr int kEpilogueWarps = 8, kBWarp = 12, kLoadWarp = 16, kMmaWarp = 19;
-    static constexpr int kThreads = 32 * 20;
-    // Registers: 96 per thread at launch; the warpgroups then share them out, 168 for the epilogue's
+    static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // 128 scale bytes per raw stage, by box and row
+    static constexpr int kBarOff = kScaleOff + kRaw * 128;
+    // rawFull, rawEmpty [kRaw]; full, empty, peerFull [kStages]; accFull, accEmpty [2]; TMEM address
+    static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 3 * kStages + 4) + 16 + 1024;
+    static constexpr int kCols = kBk + kStages * kACols;
+    static constexpr int kEpilogueWarps = 8, kBWarp = 16, kLoadWarp = 24, kMmaWarp = 27;
+    static constexpr int kThreads = 32 * 28;
+    // Registers: 72 per thread at launch; the warpgroups then share them out, 160 for the epilogue's
     // 128 sums.
-    static constexpr int kRegs = 96, kRegsEpilogue = 168, kRegsConvert = 56, kRegsIssue = 32;
-    static_assert(2 * kRegsEpilogue + 2 * kRegsConvert + kRegsIssue <= 5 * kRegs, "the shares exceed the launch's registers");
+    static constexpr int kRegs = 72, kRegsEpilogue = 160, kRegsA = 40, kRegsB = 32, kRegsIssue = 40;
+    static_assert(2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * kRegs, "the shares exceed the launch's registers");
     static_assert(kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
-    static_assert(kFlush >= 2 && kFlush % 2 == 0, "flush period");
+    static_assert(kFlush >= kTurn && kFlush % kTurn == 0 && kStages >= int(kTurn) + 2, "flushes end turns, turns overlap");
 };
 
 // kind::f16 with FP32 accumulators (bits 4-5 = 1), bf16 A and B (bits 7-9 and 10-12 = 1), B
@@ -83,16 +94,17 @@ __host__ __device__ constexpr uint32_t bf16Idesc(uint32_t m, uint32_t n) {
 }
 // D(tmem) (+)= A(tmem, bf16) x B(shared memory, bf16).
 template <int CG>
-__device__ __forceinline__ void mmaBf16Ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mmaBf16Ts(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
     if constexpr (CG == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+                     "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
                      : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+                     "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
                      : "memory");
 }
 
@@ -172,6 +184,15 @@ __device__ __forceinline__ __nv_bfloat162 scalePair(uint32_t byte) {
 // half of the quarter takes columns 0 and 1 of each four, the second half 2 and 3.
 __device__ __forceinline__ uint32_t laneColumn(uint32_t l) { return 4 * (l % 8) + 2 * (l / 16) + (l / 8) % 2; }
 
+__device__ __forceinline__ uint32_t ldsU8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void stsU8(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 // Column of dW (from the tile's first) of column c of the accumulator half h. Over a pair of CTAs an
 // MMA takes its first columns from the first CTA's shared memory, the others from the second's.
 template <int CG> __device__ __forceinline__ uint32_t columnOf(uint32_t h, uint32_t c) {
@@ -194,13 +215,14 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rawFull = base + L::kBarOff, rawEmpty = rawFull + 8 * L::kRaw;
     const uint32_t full = rawEmpty + 8 * L::kRaw, empty = full + 8 * L::kStages;
-    const uint32_t accFull = empty + 8 * L::kStages, accEmpty = accFull + 16, tmemSlot = accEmpty + 16;
+    const uint32_t peerFull = empty + 8 * L::kStages; // in the first CTA: the second's stage is full
+    const uint32_t accFull = peerFull + 8 * L::kStages, accEmpty = accFull + 16, tmemSlot = accEmpty + 16;
     const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kRaw; ++i)
-            dev::mbarInit(rawFull + 8 * i, TMA ? 1 : 3), dev::mbarInit(rawEmpty + 8 * i, 8); // warps of A and B
+            dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 3), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
         for (int i = 0; i < L::kStages; ++i)
-            dev::mbarInit(full + 8 * i, 8 * CG), dev::mbarInit(empty + 8 * i, 1);
+            dev::mbarInit(full + 8 * i, 8), dev::mbarInit(empty + 8 * i, 1), dev::mbarInit(peerFull + 8 * i, 1);
         for (int i = 0; i < 2; ++i) // of a half of the columns
             dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, 4 * CG);
         dev::fenceBarrierInit();
@@ -210,7 +232,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     dev::tcFenceBefore();
     clusterSync<CG>();
     dev::tcFenceAfter();
-    const uint32_t tmem = dev::ldsU32(tmemSlot), tmemA = tmem + 384;
+    const uint32_t tmem = dev::ldsU32(tmemSlot), tmemA = tmem + L::kBk;
     const uint32_t unit = blockIdx.x / CG, tiles = p.tilesN * p.tilesK;
     const uint32_t tile = unit % tiles, split = unit / tiles;
     const uint32_t n0 = (tile % p.tilesN * CG + rank) * 128;
@@ -218,9 +240,12 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const uint64_t begin = uint64_t(split) * p.rowsPerSplit;
     const uint64_t end = min(uint64_t(p.rows), begin + p.rowsPerSplit);
     const uint32_t stages = uint32_t((end - begin + L::kRows - 1) / L::kRows);
-    // Flush e empties accumulator e % 3, which holds half e % 2: one every kFlush / 2 stages, and two
-    // after the last stage.
-    const uint32_t flushes = stages == 0 ? 0 : (stages - 1) / (L::kFlush / 2) + 2;
+    // A half of the columns is flushed kFlush stages after its offset (half a turn for the first half,
+    // none for the second), every kFlush stages from there on, and behind the last stage.
+    auto flushCount = [&](uint32_t h) {
+        const uint32_t offset = h == 0 ? L::kTurn / 2 : 0;
+        return stages == 0 ? 0u : 1 + (stages - 1 > offset ? (stages - 1 - offset) / L::kFlush : 0);
+    };
 
     if (warp < L::kEpilogueWarps) {
         registersUp<L::kRegsEpilogue>();
@@ -230,9 +255,9 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
         for (int i = 0; i < 128; ++i)
             sum[i] = 0.0f;
         bool ok = true;
-        for (uint32_t e = half; e < flushes; e += 2) {
-            const uint32_t acc = e % 3;
-            if (!waitCluster<CG>(accFull + 8 * half, (e / 2) & 1)) {
+        const uint32_t flushes = flushCount(half);
+        for (uint32_t e = 0; e < flushes; ++e) {
+            if (!waitPhase(accFull + 8 * half, e & 1)) {
                 ok = false;
                 break;
             }
@@ -240,7 +265,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 128; c += 16) {
                 uint32_t r[16];
-                dev::tcLoad32x32bx16(tmem + acc * 128 + c + (quarter << 21), r);
+                dev::tcLoad32x32bx16(tmem + half * 128 + c + (quarter << 21), r);
                 dev::tcWaitLd();
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -279,26 +304,35 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
             }
         }
     } else if (warp < L::kBWarp) {
-        registersDown<L::kRegsConvert>();
-        // ---- A: the warp's quarter of the 128 columns of dy ----
+        registersDown<L::kRegsA>();
+        // ---- A: the warp's quarter of the 128 columns of dy; two sets of warps take alternate stages,
+        // since a warp spends more time on a stage's waits and fences than on its values ----
+        constexpr int kJ = L::kRows / 32; // 16 kJ rows at a time, for the registers
         const uint32_t quarter = warp % 4, q4 = lane % 4;
         const uint32_t byte = (32 * quarter + 4 * (lane / 4)) * sizeof(T); // of the thread's columns in a raw row
         const uint32_t from = base + L::kRawOff + byte / 128 * L::kBox, within = byte % 128;
-        uint32_t raw = 0, rawPhase = 0, s = 0, phase = 1; // a stage's first turn does not wait
-        for (uint32_t it = 0; it < stages; ++it) {
-            if (!waitPhase(rawFull + 8 * raw, rawPhase) || !waitCluster<CG>(empty + 8 * s, phase))
+        for (uint32_t it = warp / 4 % 2; it < stages; it += 2) {
+            const uint32_t raw = it % L::kRaw, s = it % L::kStages;
+            if (!waitPhase(rawFull + 8 * raw, it / L::kRaw & 1) || !waitPhase(empty + 8 * s, (it / L::kStages + 1) & 1))
                 break;
             dev::tcFenceAfter();
             const uint32_t src = from + raw * L::kRawBytes;
             const uint32_t to = tmemA + s * L::kACols + (quarter << 21);
+            // Loads in batches: the compiler keeps the order of these accesses, and a load behind a store
+            // would wait for what the store needs.
 #pragma unroll
-            for (int j = 0; j < L::kRows / 16; ++j) {
-                Quad<T> q[4]; // operand rows 16 j + 4 q4 + i
+            for (int j0 = 0; j0 < L::kRows / 16; j0 += kJ) {
+            Quad<T> quads[kJ][4]; // operand rows 16 (j0 + j) + 4 q4 + i
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = 16 * j + 8 * (i / 2) + 2 * q4 + i % 2;
-                    q[i] = loadQuad<T>(src + r * 128 + (within ^ ((r & 7) << 4)));
+                    const uint32_t r = 16 * (j0 + j) + 8 * (i / 2) + 2 * q4 + i % 2;
+                    quads[j][i] = loadQuad<T>(src + r * 128 + (within ^ ((r & 7) << 4)));
                 }
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                const Quad<T>(&q)[4] = quads[j];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t out[4][L::kP];
@@ -307,128 +341,135 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                         splitPair<T>(q[2 * (x % 2)], q[2 * (x % 2) + 1], 2 * half + x / 2, out[x]);
 #pragma unroll
                     for (int m = 0; m < L::kP; ++m)
-                        tcStore16x256b(to + m * (L::kRows / 2) + 8 * j + (half << 20), out[0][m], out[1][m], out[2][m],
+                        tcStore16x256b(to + m * (L::kRows / 2) + 8 * (j0 + j) + (half << 20), out[0][m], out[1][m], out[2][m],
                                        out[3][m]);
                 }
+            }
             }
             dev::tcWaitSt();
             dev::tcFenceBefore();
             __syncwarp();
             if (lane == 0) {
                 dev::mbarArrive(rawEmpty + 8 * raw);
-                arriveLeader<CG>(full + 8 * s);
+                dev::mbarArrive(full + 8 * s);
             }
-            if (++raw == L::kRaw)
-                raw = 0, rawPhase ^= 1;
-            if (++s == L::kStages)
-                s = 0, phase ^= 1;
         }
     } else if (warp < L::kLoadWarp) {
-        registersDown<L::kRegsConvert>();
-        // ---- B: a quarter of the stage's rows per warp, 16 lanes of 8 columns per row and box ----
+        registersDown<L::kRegsB>();
+        // ---- B: a quarter of the stage's rows per warp, 16 lanes of 8 columns per row and box; two sets
+        // of warps, as for A ----
         constexpr uint32_t kWarpRows = L::kRows / 4;
-        const uint32_t first = (warp - L::kBWarp) * kWarpRows;
-        const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock;
-        const uint32_t sRow = lane % kWarpRows, sBox = lane / kWarpRows;
-        const uint32_t sCol = kMine / kBlock + sBox;
-        const bool sMine = sBox < uint32_t(L::kBBoxes) && sCol < kBlocks;
-        auto scaleOf = [&](uint32_t it) {
-            const uint64_t r = begin + uint64_t(it) * L::kRows + first + sRow;
-            return sMine && it < stages && r < end ? uint32_t(__ldg(p.scales + r * kBlocks + sCol)) : 127u;
-        };
-        uint32_t scale0 = scaleOf(0), scale1 = scaleOf(1); // two stages ahead
-        uint32_t raw = 0, rawPhase = 0, s = 0, phase = 1;
-        for (uint32_t it = 0; it < stages; ++it) {
-            const uint32_t scales = scale0;
-            scale0 = scale1;
-            scale1 = scaleOf(it + 2);
-            if (!waitPhase(rawFull + 8 * raw, rawPhase) || !waitCluster<CG>(empty + 8 * s, phase))
+        const uint32_t first = warp % 4 * kWarpRows;
+        // No load from global memory here: the proxy fence below would wait for it.
+        for (uint32_t it = warp / 4 % 2; it < stages; it += 2) {
+            const uint32_t raw = it % L::kRaw, s = it % L::kStages;
+            if (!waitPhase(rawFull + 8 * raw, it / L::kRaw & 1) || !waitPhase(empty + 8 * s, (it / L::kStages + 1) & 1))
                 break;
+            const uint32_t scales = base + L::kScaleOff + raw * 128;
             const uint32_t src = base + L::kRawOff + raw * L::kRawBytes + L::kABoxes * L::kBox;
             const uint32_t to = base + s * L::kBBytes;
 #pragma unroll
-            for (int box = 0; box < L::kBBoxes; ++box)
+            for (int batch = 0; batch < L::kBBoxes * int(kWarpRows) / 8; ++batch) {
+                const uint32_t box = batch / (kWarpRows / 8), c = lane % 16;
+                const uint32_t r0 = first + batch % (kWarpRows / 8) * 8 + lane / 16;
+                uint2 w[4];
+                uint32_t scale[4];
 #pragma unroll
-                for (uint32_t i = 0; i < kWarpRows; i += 2) {
-                    const uint32_t local = i + lane / 16, r = first + local, c = lane % 16;
-                    const uint2 w = dev::ldsV2(src + box * L::kBox + r * 128 + 8 * c);
-                    const __nv_bfloat162 scale =
-                        scalePair(__shfl_sync(0xFFFFFFFFu, scales, local + box * kWarpRows));
+                for (uint32_t i = 0; i < 4; ++i) {
+                    w[i] = dev::ldsV2(src + box * L::kBox + (r0 + 2 * i) * 128 + 8 * c);
+                    scale[i] = ldsU8(scales + box * L::kRows + r0 + 2 * i);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const __nv_bfloat162 pair = scalePair(scale[i]);
                     uint32_t o[4];
-                    int8ToBf16(w.x, scale, o[0], o[1]);
-                    int8ToBf16(w.y, scale, o[2], o[3]);
-                    const uint32_t k = operandRow(r);
+                    int8ToBf16(w[i].x, pair, o[0], o[1]);
+                    int8ToBf16(w[i].y, pair, o[2], o[3]);
+                    const uint32_t k = operandRow(r0 + 2 * i);
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
                                  ::"r"(to + (2 * box + c / 8) * L::kBox + k * 128 + ((c ^ k) & 7) * 16), "r"(o[0]),
                                  "r"(o[1]), "r"(o[2]), "r"(o[3])
                                  : "memory");
                 }
+            }
             dev::fenceProxyAsyncShared();
             __syncwarp();
             if (lane == 0) {
                 dev::mbarArrive(rawEmpty + 8 * raw);
-                arriveLeader<CG>(full + 8 * s);
+                dev::mbarArrive(full + 8 * s);
             }
-            if (++raw == L::kRaw)
-                raw = 0, rawPhase ^= 1;
-            if (++s == L::kStages)
-                s = 0, phase ^= 1;
         }
     } else {
         registersDown<L::kRegsIssue>();
         if (warp == L::kMmaWarp) {
-            if (lane == 0 && rank == 0) {
-                // ---- MMA issue ----
-                uint32_t s = 0, phase = 0, flushed = 0;
-                uint32_t acc[2] = {0, 1};
-                bool fresh[2] = {true, true}, ok = true;
-                auto flush = [&](uint32_t h) { // the half goes on in the accumulator that was flushed before
-                    commitCluster<CG>(accFull + 8 * h);
-                    acc[h] = (flushed + 2) % 3;
-                    fresh[h] = true;
-                    ++flushed;
-                };
-                for (uint32_t it = 0; it < stages && ok; ++it) {
-                    if (!waitCluster<CG>(full + 8 * s, phase)) {
-                        ok = false;
-                        break;
-                    }
-                    dev::tcFenceAfter();
-                    const uint32_t a = tmemA + s * L::kACols;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // The accumulator of a fresh half was emptied by the flush before the half's own
-                        // last one, which the epilogue must have read out.
-                        if (fresh[h] && flushed >= 2) {
-                            const uint32_t before = flushed - 2;
-                            if (!waitCluster<CG>(accEmpty + 8 * (before % 2), (before / 2) & 1)) {
-                                ok = false;
-                                break;
-                            }
-                            dev::tcFenceAfter();
+            if (rank == 0) {
+                // ---- MMA issue, by the whole warp in uniform control flow ----
+                const uint32_t elected = electLane();
+                bool ok = true;
+                uint32_t next[2] = {0, 0}, slot[2] = {0, 0}; // next stage of each half, and its place in the ring
+                uint32_t turnEnd[2] = {L::kTurn / 2, L::kTurn}, untilFlush[2] = {L::kTurn / 2 + L::kFlush, L::kFlush};
+                uint32_t drained[2] = {0, 0}, flushes[2] = {0, 0}; // 2 + the phase to wait for before the next MMA
+                uint32_t seen = 0, seenSlot = 0, seenPhase = 0; // stages seen full
+                auto turn = [&](auto half) {
+                    constexpr uint32_t h = decltype(half)::value;
+                    uint32_t first = next[h] == 0; // the next MMA overwrites the accumulator
+                    if (drained[h] != 0 && next[h] < stages) {
+                        if (!waitCluster<CG>(accEmpty + 8 * h, drained[h] & 1)) {
+                            ok = false;
+                            return;
                         }
-                        const uint32_t b = base + s * L::kBBytes + h * (2 / CG) * L::kBox;
-                        const uint64_t desc = swizzledDesc(b, L::kBox, 1024);
+                        drained[h] = 0;
+                        first = 1;
+                    }
+                    for (; next[h] < turnEnd[h] && next[h] < stages; ++next[h]) {
+                        if (next[h] == seen) {
+                            if (!waitPhase(full + 8 * seenSlot, seenPhase) ||
+                                (CG == 2 && !waitCluster<CG>(peerFull + 8 * seenSlot, seenPhase))) {
+                                ok = false;
+                                return;
+                            }
+                            ++seen;
+                            if (++seenSlot == L::kStages)
+                                seenSlot = 0, seenPhase ^= 1;
+                        }
+                        dev::tcFenceAfter();
+                        const uint32_t s = slot[h];
+                        const uint32_t a = tmemA + s * L::kACols;
+                        const uint64_t desc = swizzledDesc(base + s * L::kBBytes + h * (2 / CG) * L::kBox, L::kBox, 1024);
 #pragma unroll
                         for (int j = 0; j < L::kRows / 16; ++j)
 #pragma unroll
-                            for (int m = 0; m < L::kP; ++m) {
-                                mmaBf16Ts<CG>(tmem + acc[h] * 128, a + m * (L::kRows / 2) + 8 * j, desc + 128 * j,
-                                              bf16Idesc(128 * CG, 128), !(fresh[h] && j == 0 && m == 0));
-                            }
-                        fresh[h] = false;
+                            for (int m = 0; m < L::kP; ++m)
+                                mmaBf16Ts<CG>(elected, tmem + h * 128, a + m * (L::kRows / 2) + 8 * j, desc + 128 * j,
+                                              bf16Idesc(128 * CG, 128), j + m != 0 ? 1u : 1u - first);
+                        first = 0;
+                        if (next[1 - h] > next[h]) // the other half was first: the stage is done with
+                            commitCluster<CG>(elected, empty + 8 * s);
+                        slot[h] = s + 1 == L::kStages ? 0 : s + 1;
+                        if (--untilFlush[h] == 0 || next[h] + 1 == stages) {
+                            commitCluster<CG>(elected, accFull + 8 * h);
+                            untilFlush[h] = L::kFlush;
+                            drained[h] = 2 + flushes[h] % 2;
+                            ++flushes[h];
+                        }
                     }
-                    if (!ok)
+                    turnEnd[h] += L::kTurn;
+                };
+                while (ok && (next[0] < stages || next[1] < stages)) {
+                    turn(Const<0>{});
+                    if (ok)
+                        turn(Const<1>{});
+                }
+            } else if (lane == 0) {
+                // ---- the second CTA of a pair passes its full stages on: one cluster-wide release
+                // per stage, instead of one in every converting warp, whose loads it would wait for ----
+                uint32_t s = 0, phase = 0;
+                for (uint32_t it = 0; it < stages; ++it) {
+                    if (!waitPhase(full + 8 * s, phase))
                         break;
-                    commitCluster<CG>(empty + 8 * s);
-                    if ((it + 1) % (L::kFlush / 2) == 0 && it + 1 < stages)
-                        flush(flushed % 2);
+                    arriveLeader<CG>(peerFull + 8 * s);
                     if (++s == L::kStages)
                         s = 0, phase ^= 1;
-                }
-                if (ok && stages != 0) {
-                    flush(flushed % 2);
-                    flush(flushed % 2);
                 }
             }
         } else if constexpr (TMA) {
@@ -458,6 +499,51 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                 if (!ok)
                     for (uint32_t i = it < L::kRaw ? 0 : it - L::kRaw; i < it; ++i)
                         waitPhase(rawFull + 8 * (i % L::kRaw), (i / L::kRaw) & 1);
+            } else if (warp != L::kLoadWarp) {
+                // ---- scale bytes: two warps take alternate stages, loaded two of their stages ahead and
+                // brought into L2 before; rows and blocks outside count 1.0 ----
+                constexpr int kLoads = L::kRows * L::kBBoxes / 32;
+                constexpr uint32_t kEarly = 12; // stages
+                const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock;
+                uint32_t held[2][kLoads];
+                auto place = [&](uint32_t it, int i, const uint8_t*& at) {
+                    const uint32_t item = 32 * i + lane, col = kMine / kBlock + item / L::kRows;
+                    const uint64_t r = begin + uint64_t(it) * L::kRows + item % L::kRows;
+                    at = p.scales + r * kBlocks + col;
+                    return r < end && col < kBlocks;
+                };
+                auto fetch = [&](uint32_t it, uint32_t (&v)[kLoads]) {
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        const uint8_t* at;
+                        v[i] = place(it, i, at) ? uint32_t(__ldg(at)) : 127u;
+                    }
+                };
+                const uint32_t first = warp - L::kLoadWarp - 1;
+                fetch(first, held[0]);
+                fetch(first + 2, held[1]);
+                bool ok = true;
+                for (uint32_t it = first; it < stages && ok; it += 4)
+#pragma unroll
+                    for (uint32_t u = 0; u < 2; ++u) {
+                        const uint32_t stage = it + 2 * u, raw = stage % L::kRaw;
+                        if (ok && stage < stages) {
+                            ok = waitPhase(rawEmpty + 8 * raw, (stage / L::kRaw + 1) & 1);
+#pragma unroll
+                            for (int i = 0; i < kLoads; ++i)
+                                stsU8(base + L::kScaleOff + raw * 128 + 32 * i + lane, held[u][i]);
+                            __syncwarp();
+                            if (lane == 0)
+                                dev::mbarArrive(rawFull + 8 * raw);
+                            fetch(stage + 4, held[u]);
+#pragma unroll
+                            for (int i = 0; i < kLoads; ++i) {
+                                const uint8_t* at;
+                                if (place(stage + kEarly, i, at))
+                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                            }
+                        }
+                    }
             }
         } else {
             // ---- raw stages element by element, for rows that do not start on 16 bytes: three warps ----
@@ -481,11 +567,15 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                             asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
                         }
                     }
+                    if (lane < uint32_t(L::kBBoxes)) {
+                        const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, col = kMine / kBlock + lane;
+                        stsU8(base + L::kScaleOff + raw * 128 + lane * L::kRows + r,
+                              in && col < kBlocks ? uint32_t(__ldg(p.scales + row * kBlocks + col)) : 127u);
+                    }
                     const uint8_t* q = p.q + row * p.qStride + kMine;
                     for (uint32_t c = lane; c < uint32_t(L::kBCols); c += 32) {
                         const uint32_t at = to + (L::kABoxes + c / 128) * L::kBox + r * 128 + c % 128;
-                        const unsigned short v = in && kMine + c < p.k ? __ldg(q + c) : 0;
-                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+                        stsU8(at, in && kMine + c < p.k ? uint32_t(__ldg(q + c)) : 0u);
                     }
                 }
                 __syncwarp();
