@@ -97,7 +97,14 @@ __device__ __forceinline__ void mmaScaled8(uint32_t elected, uint32_t d, uint64_
                      : "memory");
 }
 
-// Warp load of 32 TMEM lanes x 32 columns: thread t reads lane t, r[j] = column j.
+// Warp load of 32 TMEM lanes x 8 columns: thread t reads lane t, r[j] = column j.
+__device__ __forceinline__ void tcLoad32x32bx8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+// The same for 32 columns: thread t reads lane t, r[j] = column j.
 __device__ __forceinline__ void tcLoad32x32bx32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -126,40 +133,17 @@ template <int CG> __device__ __forceinline__ void clusterSync() {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
-// Arrive on the barrier at this address of the cluster's first CTA.
+// Arrive on the barrier at this address of the cluster's first CTA. No cluster-wide release, which
+// took about 1300 cycles and held the MMAs up: nothing that one CTA wrote is read by the other. Each
+// SM's tensor core reads its own CTA's shared and tensor memory, whose writers have fenced and
+// arrived before; the arrival only tells the issuing thread so.
 template <int CG> __device__ __forceinline__ void arriveLeader(uint32_t bar) {
     if constexpr (CG == 1)
         dev::mbarArrive(bar);
     else
         asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-                     "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+                     "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
                      : "memory");
-}
-// waitPhase for a barrier on which the other CTA of the cluster arrives too.
-template <int CG> __device__ __forceinline__ bool waitCluster(uint32_t bar, uint32_t parity) {
-    if constexpr (CG == 1)
-        return waitPhase(bar, parity);
-    uint64_t start = 0;
-    for (uint32_t attempt = 1;; ++attempt) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done)
-                     : "r"(bar), "r"(parity), "r"(2000u)
-                     : "memory");
-        if (done)
-            return true;
-        if ((attempt & 63u) == 0) {
-            const uint64_t now = dev::globalTimerNs();
-            if (start == 0) {
-                start = now;
-            } else if (now - start > kDenseWaitNs) {
-                atomicOr(&gDenseStatus, 1u);
-                return false;
-            }
-        }
-    }
 }
 // One arrival on the barrier at this address in every CTA of the cluster, once the tcgen05
 // operations that the elected lane issued are done.

@@ -72,16 +72,17 @@ template <typename T, int CG> struct GradTile {
     static constexpr uint32_t kTurn = kStages >= 6 ? 4 : 2;               // stages of a half in one go
     static constexpr uint32_t kFlush = 60 / kSteps / kTurn * kTurn;        // stages between two flushes of a half
     static constexpr int kRawOff = kStages * kBBytes;
-    static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // 128 scale bytes per raw stage, by box and row
-    static constexpr int kBarOff = kScaleOff + kRaw * 128;
+    static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // a raw stage's scales as bf16 pairs, by box and row
+    static constexpr int kScaleBytes = kRows * kBBoxes * 4;
+    static constexpr int kBarOff = kScaleOff + kRaw * kScaleBytes;
     // rawFull, rawEmpty [kRaw]; full, empty, peerFull [kStages]; accFull, accEmpty [2]; TMEM address
     static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 3 * kStages + 4) + 16 + 1024;
     static constexpr int kCols = kBk + kStages * kACols;
     static constexpr int kEpilogueWarps = 8, kBWarp = 16, kLoadWarp = 24, kMmaWarp = 27;
     static constexpr int kThreads = 32 * 28;
-    // Registers: 72 per thread at launch; the warpgroups then share them out, 160 for the epilogue's
+    // Registers: 72 per thread at launch; the warpgroups then share them out, 152 for the epilogue's
     // 128 sums.
-    static constexpr int kRegs = 72, kRegsEpilogue = 160, kRegsA = 40, kRegsB = 32, kRegsIssue = 40;
+    static constexpr int kRegs = 72, kRegsEpilogue = 152, kRegsA = 40, kRegsB = 40, kRegsIssue = 40;
     static_assert(2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * kRegs, "the shares exceed the launch's registers");
     static_assert(kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
     static_assert(kFlush >= kTurn && kFlush % kTurn == 0 && kStages >= int(kTurn) + 2, "flushes end turns, turns overlap");
@@ -158,25 +159,24 @@ template <typename T> __device__ __forceinline__ void splitPair(const Quad<T>& u
     }
 }
 
-// Four INT8 elements times a power of two (as a bf16 pair) in bf16: low 7 bits under the exponent
+// Four INT8 elements times a power of two (a bf16 pair) in bf16: low 7 bits under the exponent
 // of 128, minus 128 or, for negative elements, 256. Every step is exact.
-__device__ __forceinline__ void int8ToBf16(uint32_t w, __nv_bfloat162 scale, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void int8ToBf16(uint32_t w, uint32_t scale, uint32_t& lo, uint32_t& hi) {
     const uint32_t x[2] = {__byte_perm(w, 0u, 0x4140), __byte_perm(w, 0u, 0x4342)};
     uint32_t out[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint32_t v = (x[i] & 0x007F007Fu) | 0x43004300u, c = (x[i] & 0x00800080u) | 0xC300C300u;
         const __nv_bfloat162 f = __hmul2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                                 *reinterpret_cast<const __nv_bfloat162*>(&c)), scale);
+                                                 *reinterpret_cast<const __nv_bfloat162*>(&c)),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&scale));
         out[i] = *reinterpret_cast<const uint32_t*>(&f);
     }
     lo = out[0], hi = out[1];
 }
 // 2^e of a scale byte as a bf16 pair (NaN for 255, a subnormal for 0).
-__device__ __forceinline__ __nv_bfloat162 scalePair(uint32_t byte) {
-    const uint32_t h = byte == 255u ? 0x7FC0u : byte == 0u ? 0x0040u : byte << 7;
-    const uint32_t w = h * 0x10001u;
-    return *reinterpret_cast<const __nv_bfloat162*>(&w);
+__device__ __forceinline__ uint32_t scalePair(uint32_t byte) {
+    return (byte == 255u ? 0x7FC0u : byte == 0u ? 0x0040u : byte << 7) * 0x10001u;
 }
 
 // Lane of a 32-lane quarter of A and D -> column of dy within the quarter's 32: the 16-lane store
@@ -184,10 +184,8 @@ __device__ __forceinline__ __nv_bfloat162 scalePair(uint32_t byte) {
 // half of the quarter takes columns 0 and 1 of each four, the second half 2 and 3.
 __device__ __forceinline__ uint32_t laneColumn(uint32_t l) { return 4 * (l % 8) + 2 * (l / 16) + (l / 8) % 2; }
 
-__device__ __forceinline__ uint32_t ldsU8(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void stsU32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void stsU8(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
@@ -263,12 +261,12 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
             }
             dev::tcFenceAfter();
 #pragma unroll
-            for (int c = 0; c < 128; c += 16) {
-                uint32_t r[16];
-                dev::tcLoad32x32bx16(tmem + half * 128 + c + (quarter << 21), r);
+            for (int c = 0; c < 128; c += 8) {
+                uint32_t r[8];
+                tcLoad32x32bx8(tmem + half * 128 + c + (quarter << 21), r);
                 dev::tcWaitLd();
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+                for (int i = 0; i < 8; ++i)
                     sum[c + i] += __uint_as_float(r[i]);
             }
             dev::tcFenceBefore();
@@ -359,36 +357,37 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
         // ---- B: a quarter of the stage's rows per warp, 16 lanes of 8 columns per row and box; two sets
         // of warps, as for A ----
         constexpr uint32_t kWarpRows = L::kRows / 4;
-        const uint32_t first = warp % 4 * kWarpRows;
+        const uint32_t c = lane % 16, row0 = warp % 4 * kWarpRows + lane / 16;
         // No load from global memory here: the proxy fence below would wait for it.
         for (uint32_t it = warp / 4 % 2; it < stages; it += 2) {
             const uint32_t raw = it % L::kRaw, s = it % L::kStages;
             if (!waitPhase(rawFull + 8 * raw, it / L::kRaw & 1) || !waitPhase(empty + 8 * s, (it / L::kStages + 1) & 1))
                 break;
-            const uint32_t scales = base + L::kScaleOff + raw * 128;
+            const uint32_t scales = base + L::kScaleOff + raw * L::kScaleBytes;
             const uint32_t src = base + L::kRawOff + raw * L::kRawBytes + L::kABoxes * L::kBox;
             const uint32_t to = base + s * L::kBBytes;
 #pragma unroll
             for (int batch = 0; batch < L::kBBoxes * int(kWarpRows) / 8; ++batch) {
-                const uint32_t box = batch / (kWarpRows / 8), c = lane % 16;
-                const uint32_t r0 = first + batch % (kWarpRows / 8) * 8 + lane / 16;
+                const uint32_t box = batch / (kWarpRows / 8), r0 = row0 + batch % (kWarpRows / 8) * 8;
                 uint2 w[4];
                 uint32_t scale[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
                     w[i] = dev::ldsV2(src + box * L::kBox + (r0 + 2 * i) * 128 + 8 * c);
-                    scale[i] = ldsU8(scales + box * L::kRows + r0 + 2 * i);
+                    scale[i] = dev::ldsU32(scales + 4 * (box * L::kRows + r0 + 2 * i));
                 }
+                // Rows r0 + 2 i stand at operand rows k + 4 i, k = operandRow(r0), so their pieces lie 512
+                // bytes apart, in one of two swizzled places.
+                const uint32_t k = operandRow(r0), piece = (c ^ k) & 7;
+                const uint32_t at = to + (2 * box + c / 8) * L::kBox + k * 128;
+                const uint32_t even = at + piece * 16, odd = at + 512 + (piece ^ 4) * 16;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    const __nv_bfloat162 pair = scalePair(scale[i]);
                     uint32_t o[4];
-                    int8ToBf16(w[i].x, pair, o[0], o[1]);
-                    int8ToBf16(w[i].y, pair, o[2], o[3]);
-                    const uint32_t k = operandRow(r0 + 2 * i);
+                    int8ToBf16(w[i].x, scale[i], o[0], o[1]);
+                    int8ToBf16(w[i].y, scale[i], o[2], o[3]);
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(to + (2 * box + c / 8) * L::kBox + k * 128 + ((c ^ k) & 7) * 16), "r"(o[0]),
-                                 "r"(o[1]), "r"(o[2]), "r"(o[3])
+                                 ::"r"((i % 2 ? odd : even) + i / 2 * 1024), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
                                  : "memory");
                 }
             }
@@ -414,7 +413,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                     constexpr uint32_t h = decltype(half)::value;
                     uint32_t first = next[h] == 0; // the next MMA overwrites the accumulator
                     if (drained[h] != 0 && next[h] < stages) {
-                        if (!waitCluster<CG>(accEmpty + 8 * h, drained[h] & 1)) {
+                        if (!waitPhase(accEmpty + 8 * h, drained[h] & 1)) {
                             ok = false;
                             return;
                         }
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                     for (; next[h] < turnEnd[h] && next[h] < stages; ++next[h]) {
                         if (next[h] == seen) {
                             if (!waitPhase(full + 8 * seenSlot, seenPhase) ||
-                                (CG == 2 && !waitCluster<CG>(peerFull + 8 * seenSlot, seenPhase))) {
+                                (CG == 2 && !waitPhase(peerFull + 8 * seenSlot, seenPhase))) {
                                 ok = false;
                                 return;
                             }
@@ -461,8 +460,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                         turn(Const<1>{});
                 }
             } else if (lane == 0) {
-                // ---- the second CTA of a pair passes its full stages on: one cluster-wide release
-                // per stage, instead of one in every converting warp, whose loads it would wait for ----
+                // ---- the second CTA of a pair passes its full stages on ----
                 uint32_t s = 0, phase = 0;
                 for (uint32_t it = 0; it < stages; ++it) {
                     if (!waitPhase(full + 8 * s, phase))
@@ -531,7 +529,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                             ok = waitPhase(rawEmpty + 8 * raw, (stage / L::kRaw + 1) & 1);
 #pragma unroll
                             for (int i = 0; i < kLoads; ++i)
-                                stsU8(base + L::kScaleOff + raw * 128 + 32 * i + lane, held[u][i]);
+                                stsU32(base + L::kScaleOff + raw * L::kScaleBytes + 4 * (32 * i + lane), scalePair(held[u][i]));
                             __syncwarp();
                             if (lane == 0)
                                 dev::mbarArrive(rawFull + 8 * raw);
@@ -569,8 +567,8 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                     }
                     if (lane < uint32_t(L::kBBoxes)) {
                         const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, col = kMine / kBlock + lane;
-                        stsU8(base + L::kScaleOff + raw * 128 + lane * L::kRows + r,
-                              in && col < kBlocks ? uint32_t(__ldg(p.scales + row * kBlocks + col)) : 127u);
+                        stsU32(base + L::kScaleOff + raw * L::kScaleBytes + 4 * (lane * L::kRows + r),
+                               scalePair(in && col < kBlocks ? uint32_t(__ldg(p.scales + row * kBlocks + col)) : 127u));
                     }
                     const uint8_t* q = p.q + row * p.qStride + kMine;
                     for (uint32_t c = lane; c < uint32_t(L::kBCols); c += 32) {
