@@ -18,9 +18,9 @@
 //
 // The tensor core cuts off what an addition shifts out below the accumulator's last bit, about
 // 1.5e-8 of the sum for every MMA (measured; 2.1e-5 after 1300), so the accumulator is emptied every
-// 48 to 60 MMAs into fp32 registers, which round to nearest. The two halves of the 256 columns are
-// issued in turns of kTurn stages, half a turn apart: eight warps read one half out while the other's
-// turn runs.
+// 60 MMAs into the fp32 registers of eight warps, which round to nearest. The MMAs wait meanwhile:
+// halves of the accumulator that take turns need MMAs of 128 columns, which ran at 91 cycles instead
+// of 64.
 #include "dense8.cuh"
 #include "dense8_tc.cuh"
 
@@ -68,15 +68,14 @@ template <typename T, int CG> struct GradTile {
     static constexpr int kRawBytes = (kABoxes + kBBoxes) * kBox;
     static constexpr int kBBytes = kRows * kBCols * 2;
     static constexpr int kACols = kP * kRows / 2;       // tensor-memory columns of a stage of A
-    static constexpr int kSteps = kP * kRows / 16;      // MMAs per stage and accumulator
-    static constexpr uint32_t kTurn = kStages >= 6 ? 4 : 2;               // stages of a half in one go
-    static constexpr uint32_t kFlush = 60 / kSteps / kTurn * kTurn;        // stages between two flushes of a half
+    static constexpr int kSteps = kP * kRows / 16;      // MMAs per stage
+    static constexpr uint32_t kFlush = 60 / kSteps;     // stages between two flushes
     static constexpr int kRawOff = kStages * kBBytes;
     static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // a raw stage's scales as bf16 pairs, by box and row
     static constexpr int kScaleBytes = kRows * kBBoxes * 4;
     static constexpr int kBarOff = kScaleOff + kRaw * kScaleBytes;
-    // rawFull, rawEmpty [kRaw]; full, empty, peerFull [kStages]; accFull, accEmpty [2]; TMEM address
-    static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 3 * kStages + 4) + 16 + 1024;
+    // rawFull, rawEmpty [kRaw]; full, empty, peerFull [kStages]; accFull, accEmpty; TMEM address
+    static constexpr int kBytes = kBarOff + 8 * (2 * kRaw + 3 * kStages + 2) + 16 + 1024;
     static constexpr int kCols = kBk + kStages * kACols;
     static constexpr int kEpilogueWarps = 8, kBWarp = 16, kLoadWarp = 24, kMmaWarp = 27;
     static constexpr int kThreads = 32 * 28;
@@ -85,7 +84,6 @@ template <typename T, int CG> struct GradTile {
     static constexpr int kRegs = 72, kRegsEpilogue = 152, kRegsA = 40, kRegsB = 40, kRegsIssue = 40;
     static_assert(2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * kRegs, "the shares exceed the launch's registers");
     static_assert(kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
-    static_assert(kFlush >= kTurn && kFlush % kTurn == 0 && kStages >= int(kTurn) + 2, "flushes end turns, turns overlap");
 };
 
 // kind::f16 with FP32 accumulators (bits 4-5 = 1), bf16 A and B (bits 7-9 and 10-12 = 1), B
@@ -191,12 +189,6 @@ __device__ __forceinline__ void stsU8(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// Column of dW (from the tile's first) of column c of the accumulator half h. Over a pair of CTAs an
-// MMA takes its first columns from the first CTA's shared memory, the others from the second's.
-template <int CG> __device__ __forceinline__ uint32_t columnOf(uint32_t h, uint32_t c) {
-    return CG == 1 ? 128 * h + c : 64 * h + c % 64 + c / 64 * 128;
-}
-
 // Row of a raw stage whose values stand at row k of the operands. Any order will do that A and B
 // share; this one lets the four threads that read one column group of dy take rows two apart, which
 // the TMA swizzle puts into distinct banks.
@@ -214,15 +206,14 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const uint32_t rawFull = base + L::kBarOff, rawEmpty = rawFull + 8 * L::kRaw;
     const uint32_t full = rawEmpty + 8 * L::kRaw, empty = full + 8 * L::kStages;
     const uint32_t peerFull = empty + 8 * L::kStages; // in the first CTA: the second's stage is full
-    const uint32_t accFull = peerFull + 8 * L::kStages, accEmpty = accFull + 16, tmemSlot = accEmpty + 16;
+    const uint32_t accFull = peerFull + 8 * L::kStages, accEmpty = accFull + 8, tmemSlot = accEmpty + 8;
     const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kRaw; ++i)
             dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 3), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
         for (int i = 0; i < L::kStages; ++i)
             dev::mbarInit(full + 8 * i, 8), dev::mbarInit(empty + 8 * i, 1), dev::mbarInit(peerFull + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) // of a half of the columns
-            dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, 4 * CG);
+        dev::mbarInit(accFull, 1), dev::mbarInit(accEmpty, 8 * CG);
         dev::fenceBarrierInit();
     }
     if (warp == L::kMmaWarp)
@@ -238,13 +229,6 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const uint64_t begin = uint64_t(split) * p.rowsPerSplit;
     const uint64_t end = min(uint64_t(p.rows), begin + p.rowsPerSplit);
     const uint32_t stages = uint32_t((end - begin + L::kRows - 1) / L::kRows);
-    // A half of the columns is flushed kFlush stages after its offset (half a turn for the first half,
-    // none for the second), every kFlush stages from there on, and behind the last stage.
-    auto flushCount = [&](uint32_t h) {
-        const uint32_t offset = h == 0 ? L::kTurn / 2 : 0;
-        return stages == 0 ? 0u : 1 + (stages - 1 > offset ? (stages - 1 - offset) / L::kFlush : 0);
-    };
-
     if (warp < L::kEpilogueWarps) {
         registersUp<L::kRegsEpilogue>();
         const uint32_t quarter = warp % 4, half = warp / 4;
@@ -253,9 +237,9 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
         for (int i = 0; i < 128; ++i)
             sum[i] = 0.0f;
         bool ok = true;
-        const uint32_t flushes = flushCount(half);
+        const uint32_t flushes = (stages + L::kFlush - 1) / L::kFlush;
         for (uint32_t e = 0; e < flushes; ++e) {
-            if (!waitPhase(accFull + 8 * half, e & 1)) {
+            if (!waitPhase(accFull, e & 1)) {
                 ok = false;
                 break;
             }
@@ -272,7 +256,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
             dev::tcFenceBefore();
             __syncwarp();
             if (lane == 0)
-                arriveLeader<CG>(accEmpty + 8 * half);
+                arriveLeader<CG>(accEmpty);
         }
         const uint32_t row = n0 + 32 * quarter + laneColumn(lane);
         if (ok && p.partials != nullptr) {
@@ -284,7 +268,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
         } else if (ok && row < p.n) {
 #pragma unroll
             for (int i = 0; i < 128; i += 4) {
-                const uint32_t col = k0 + columnOf<CG>(half, i);
+                const uint32_t col = k0 + 128 * half + i;
                 float* out = p.dw + row * p.dwStride + col;
                 if (p.dwVector && col + 4 <= p.k) {
                     float4 v = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
@@ -404,60 +388,32 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
             if (rank == 0) {
                 // ---- MMA issue, by the whole warp in uniform control flow ----
                 const uint32_t elected = electLane();
-                bool ok = true;
-                uint32_t next[2] = {0, 0}, slot[2] = {0, 0}; // next stage of each half, and its place in the ring
-                uint32_t turnEnd[2] = {L::kTurn / 2, L::kTurn}, untilFlush[2] = {L::kTurn / 2 + L::kFlush, L::kFlush};
-                uint32_t drained[2] = {0, 0}, flushes[2] = {0, 0}; // 2 + the phase to wait for before the next MMA
-                uint32_t seen = 0, seenSlot = 0, seenPhase = 0; // stages seen full
-                auto turn = [&](auto half) {
-                    constexpr uint32_t h = decltype(half)::value;
-                    uint32_t first = next[h] == 0; // the next MMA overwrites the accumulator
-                    if (drained[h] != 0 && next[h] < stages) {
-                        if (!waitPhase(accEmpty + 8 * h, drained[h] & 1)) {
-                            ok = false;
-                            return;
-                        }
-                        drained[h] = 0;
-                        first = 1;
-                    }
-                    for (; next[h] < turnEnd[h] && next[h] < stages; ++next[h]) {
-                        if (next[h] == seen) {
-                            if (!waitPhase(full + 8 * seenSlot, seenPhase) ||
-                                (CG == 2 && !waitPhase(peerFull + 8 * seenSlot, seenPhase))) {
-                                ok = false;
-                                return;
-                            }
-                            ++seen;
-                            if (++seenSlot == L::kStages)
-                                seenSlot = 0, seenPhase ^= 1;
-                        }
-                        dev::tcFenceAfter();
-                        const uint32_t s = slot[h];
-                        const uint32_t a = tmemA + s * L::kACols;
-                        const uint64_t desc = swizzledDesc(base + s * L::kBBytes + h * (2 / CG) * L::kBox, L::kBox, 1024);
+                uint32_t slot = 0, phase = 0, untilFlush = L::kFlush, flushes = 0;
+                bool fresh = true; // the next MMA overwrites the accumulator
+                for (uint32_t x = 0; x < stages; ++x) {
+                    if (!waitPhase(full + 8 * slot, phase) || (CG == 2 && !waitPhase(peerFull + 8 * slot, phase)))
+                        break;
+                    if (fresh && flushes != 0 && !waitPhase(accEmpty, (flushes - 1) & 1))
+                        break;
+                    dev::tcFenceAfter();
+                    const uint32_t a = tmemA + slot * L::kACols;
+                    const uint64_t desc = swizzledDesc(base + slot * L::kBBytes, L::kBox, 1024);
 #pragma unroll
-                        for (int j = 0; j < L::kRows / 16; ++j)
+                    for (int j = 0; j < L::kRows / 16; ++j)
 #pragma unroll
-                            for (int m = 0; m < L::kP; ++m)
-                                mmaBf16Ts<CG>(elected, tmem + h * 128, a + m * (L::kRows / 2) + 8 * j, desc + 128 * j,
-                                              bf16Idesc(128 * CG, 128), j + m != 0 ? 1u : 1u - first);
-                        first = 0;
-                        if (next[1 - h] > next[h]) // the other half was first: the stage is done with
-                            commitCluster<CG>(elected, empty + 8 * s);
-                        slot[h] = s + 1 == L::kStages ? 0 : s + 1;
-                        if (--untilFlush[h] == 0 || next[h] + 1 == stages) {
-                            commitCluster<CG>(elected, accFull + 8 * h);
-                            untilFlush[h] = L::kFlush;
-                            drained[h] = 2 + flushes[h] % 2;
-                            ++flushes[h];
-                        }
+                        for (int m = 0; m < L::kP; ++m)
+                            mmaBf16Ts<CG>(elected, tmem, a + m * (L::kRows / 2) + 8 * j, desc + 128 * j,
+                                          bf16Idesc(128 * CG, 256), j + m != 0 ? 1u : uint32_t(!fresh));
+                    fresh = false;
+                    commitCluster<CG>(elected, empty + 8 * slot);
+                    if (++slot == L::kStages)
+                        slot = 0, phase ^= 1;
+                    if (--untilFlush == 0 || x + 1 == stages) {
+                        commitCluster<CG>(elected, accFull);
+                        untilFlush = L::kFlush;
+                        fresh = true;
+                        ++flushes;
                     }
-                    turnEnd[h] += L::kTurn;
-                };
-                while (ok && (next[0] < stages || next[1] < stages)) {
-                    turn(Const<0>{});
-                    if (ok)
-                        turn(Const<1>{});
                 }
             } else if (lane == 0) {
                 // ---- the second CTA of a pair passes its full stages on ----
@@ -620,7 +576,7 @@ __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t sp
     }
     const uint32_t l = within % 128, c = within / 128 * 4, tile = cta / CG;
     const uint32_t row = (tile % p.tilesN * CG + cta % CG) * 128 + l / 32 * 32 + laneColumn(l % 32);
-    const uint32_t col = tile / p.tilesN * 256 + columnOf<CG>(c / 128, c % 128);
+    const uint32_t col = tile / p.tilesN * 256 + c;
     if (row >= p.n || col >= p.k)
         return;
     float* out = p.dw + row * p.dwStride + col;
