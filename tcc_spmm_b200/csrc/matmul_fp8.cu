@@ -99,41 +99,49 @@ template <typename T> void launchGeneric(const Product& p) {
 }
 
 // ---- tensor cores -------------------------------------------------------------------------------
-// One CTA per SM computes tiles of 128 x BN outputs. A warp issues TMA copies of 128 bytes of k per
-// stage (128-byte swizzle); one thread issues tcgen05.mma kind::mxf8f6f4, whose E8M0 scales are the
-// blocks' own bytes: the hardware takes one scale per 32 elements of k, and a block's four groups
-// take the same one, so no scale is applied outside the tensor core and the sum over all of k stays
-// in one FP32 accumulator in tensor memory. Scales travel as words of four consecutive blocks per
-// row, loaded by a warp of their own, copied to tensor memory by the MMA thread and picked by the
-// byte selector of the instruction descriptor. Eight warps store finished tiles.
-template <int BN, bool KN> struct Tile {
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+// Persistent clusters of CG CTAs (one per SM) compute tiles of 128 CG x BN outputs. A warp issues TMA
+// copies of 128 bytes of k per stage (128-byte swizzle); one thread issues tcgen05.mma kind::mxf8f6f4,
+// over the pair where CG = 2 (each CTA brings half of b's rows, which halves what an SM reads). Its
+// E8M0 scales are the blocks' own bytes: the hardware takes one scale per 32 elements of k, and a
+// block's four groups take the same one, so no scale is applied outside the tensor core and the sum
+// over all of k stays in one FP32 accumulator in tensor memory. Scales travel as words of four
+// consecutive blocks per row, loaded by a warp of their own, copied to tensor memory by the MMA thread
+// and picked by the byte selector of the instruction descriptor. Eight warps bring finished tiles into
+// registers, release the accumulator, and write them by TMA through 4 KB of shared memory each.
+template <int BN_, int CG_> struct Tile {
+    static constexpr int BN = BN_, CG = CG_;
+    static constexpr int kStages = BN == 256 ? 5 : BN == 128 ? 4 : 6;
     static constexpr int kAcc = BN == 256 ? 1 : 2;       // accumulators in tensor memory
     static constexpr int kSlots = 4;                     // groups of four blocks' scales
     static constexpr int kSlabs = 1 + (BN + 127) / 128;  // of 512 bytes: A's rows, B's rows
-    static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
+    static constexpr int kBRows = BN / CG;               // rows of b in this CTA
+    static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kScaleOff = kStages * kStageBytes;
-    static constexpr int kBarOff = kScaleOff + kSlots * kSlabs * 512;
-    // full, empty [kStages]; scaleFull, scaleEmpty [kSlots]; accFull, accEmpty [kAcc]; TMEM address
-    static constexpr int kBars = 2 * kStages + 2 * kSlots + 2 * kAcc;
-    static constexpr int kBytes = kBarOff + 8 * kBars + 16 + 1024; // + alignment to 1024
-    static constexpr int kScaleCols = 4 * kSlabs;
-    static constexpr int kCols = kAcc * BN + kSlots * kScaleCols;
-    static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+    static constexpr int kHalf = BN / 2;                 // columns per epilogue warp
+    static constexpr int kOutBufs = BN == 256 ? 1 : 2;   // of 4 KB per epilogue warp
     static constexpr int kEpilogueWarps = 8;
+    static constexpr int kOutOff = kStages * kStageBytes;
+    static constexpr int kScaleOff = kOutOff + kEpilogueWarps * kOutBufs * 4096;
+    static constexpr int kBiasOff = kScaleOff + kSlots * kSlabs * 512; // kHalf floats per epilogue warp
+    static constexpr int kBarOff = kBiasOff + kEpilogueWarps * kHalf * 4;
+    // full, empty, peerFull [kStages]; scaleFull, scaleEmpty [kSlots]; accFull, accEmpty [kAcc]; TMEM address
+    static constexpr int kBars = 3 * kStages + 2 * kSlots + 2 * kAcc;
+    static constexpr int kNeed = kBarOff + 8 * kBars + 16 + 1024; // + alignment to 1024
+    // At least half of the shared memory: a second CTA on the SM would wait for tensor memory.
+    static constexpr int kBytes = kNeed > 120 * 1024 ? kNeed : 120 * 1024;
+    static constexpr int kScaleCols = 4 * kSlabs;
+    static constexpr int kTmemCols = 512;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
     static constexpr int kThreads = 32 * 11;
-    static_assert(kCols <= 512 && kBytes <= 232448, "resources");
-    static_assert(!KN || BN >= 128, "rows of a [k, n] operand are copied 128 bytes at a time");
+    static_assert(kAcc * BN + kSlots * kScaleCols <= kTmemCols && kBytes <= 232448, "resources");
 };
 
 // Instruction descriptor of kind::mxf8f6f4 without the byte selectors: types (0 e4m3, 1 e5m2) in
 // bits 7-9 and 10-12, B MN-major in bit 16, N / 8 in bits 17-22, E8M0 scales in bit 23, M / 128 in
 // bits 27-28. The selectors are bits 29-30 (A) and 4-5 (B).
-__host__ __device__ constexpr uint32_t scaledIdesc(bool aE5m2, bool bE5m2, bool kn, uint32_t n) {
+__host__ __device__ constexpr uint32_t scaledIdesc(bool aE5m2, bool bE5m2, bool kn, uint32_t m, uint32_t n) {
     return (uint32_t(aE5m2) << 7) | (uint32_t(bE5m2) << 10) | (uint32_t(kn) << 16) | ((n >> 3) << 17) | (1u << 23) |
-           (1u << 27);
+           ((m >> 7) << 27);
 }
 
 struct ScaleView {
@@ -147,7 +155,8 @@ struct ProductArgs {
     const float* bias;
     void* out;
     uint64_t outStride;
-    int outType, outAlign; // outAlign: 32, 16 or 0 bytes that every output row starts on
+    int outType;
+    bool outTma; // output rows start on 16 bytes: written by TMA
     uint32_t m, n, k, tilesM, tilesN;
     uint32_t idesc;
 };
@@ -178,119 +187,136 @@ __device__ __forceinline__ uint32_t scaleWordKn(const ScaleView& s, uint32_t kBl
 }
 
 // Tiles in groups of 16 rows of tiles, so that the tiles in flight share operands in L2.
-__device__ __forceinline__ void tilePlace(const ProductArgs& p, uint32_t t, uint64_t& m0, uint32_t& n0, uint32_t bn) {
+template <typename L> __device__ __forceinline__ void tilePlace(const ProductArgs& p, uint32_t t, uint64_t& m0, uint32_t& n0) {
     const uint32_t span = 16 * p.tilesN;
     const uint32_t first = t / span * 16, local = t % span;
     const uint32_t height = min(16u, p.tilesM - first);
-    m0 = uint64_t(first + local % height) * 128;
-    n0 = local / height * bn;
+    m0 = uint64_t(first + local % height) * (128 * L::CG);
+    n0 = local / height * L::BN;
 }
 
-__device__ __forceinline__ void storeGlobal32(void* p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-
-// 16 columns of one output row from column c on.
+// A tensor-memory row's columns [c, c + N) with the bias added, to 16 bytes of T each.
 template <typename T>
-__device__ __forceinline__ void storeColumns16(const ProductArgs& p, uint64_t row, uint32_t c, const uint32_t* acc) {
-    if (c >= p.n)
-        return;
-    T* out = static_cast<T*>(p.out) + row * p.outStride + c;
-    float v[16];
+__device__ __forceinline__ uint4 outputPiece(const uint32_t* acc, uint32_t bias) {
+    constexpr int kE = kPer16<T>;
+    float v[kE];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        v[i] = __uint_as_float(acc[i]) + (p.bias && c + i < p.n ? __ldg(p.bias + c + i) : 0.0f);
-    if (p.outAlign != 0 && c + 16 <= p.n) {
-        constexpr int kE = kPer16<T>;
-        uint4 w[16 / kE];
+    for (int i = 0; i < kE; i += 4) {
+        const uint4 b = dev::ldsV4(bias + 4 * i);
+        v[i] = __uint_as_float(acc[i]) + __uint_as_float(b.x), v[i + 1] = __uint_as_float(acc[i + 1]) + __uint_as_float(b.y);
+        v[i + 2] = __uint_as_float(acc[i + 2]) + __uint_as_float(b.z), v[i + 3] = __uint_as_float(acc[i + 3]) + __uint_as_float(b.w);
+    }
+    return pack16<T>(v);
+}
+
+__device__ __forceinline__ void tmaStore2d(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int LEFT> __device__ __forceinline__ void tmaStoreWaitRead() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+
+// One warp's 32 rows x kHalf columns of a finished tile: lane = row. Boxes of 32 rows x 128 bytes (or
+// the whole width, if less) go through shared memory, swizzled as the map says, to the output; rows
+// that TMA cannot write go straight from the registers.
+template <typename L, typename T>
+__device__ __forceinline__ void storeTile(const ProductArgs& p, const CUtensorMap* map, const uint32_t (&r)[L::kHalf],
+                                          uint32_t buf, uint32_t bias, uint64_t row0, uint32_t n0, uint32_t lane) {
+    constexpr int kWidth = L::kHalf * int(sizeof(T)) < 128 ? L::kHalf * int(sizeof(T)) : 128;
+    constexpr int kPerBox = kWidth / int(sizeof(T)), kBoxes = L::kHalf / kPerBox;
+    if (p.outTma) {
 #pragma unroll
-        for (int i = 0; i < 16 / kE; ++i) {
-            float part[kE];
+        for (int box = 0; box < kBoxes; ++box) {
+            if (n0 + box * kPerBox >= p.n)
+                break;
+            const uint32_t at = buf + box % L::kOutBufs * 4096;
+            if (lane == 0) // the box that was stored from here before has been read
+                tmaStoreWaitRead<L::kOutBufs - 1>();
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < kE; ++e)
-                part[e] = v[kE * i + e];
-            w[i] = pack16<T>(part);
-        }
-        if (p.outAlign == 32) {
-#pragma unroll
-            for (int i = 0; i < 16 / kE; i += 2) {
-                const uint32_t u[8] = {w[i].x, w[i].y, w[i].z, w[i].w, w[i + 1].x, w[i + 1].y, w[i + 1].z, w[i + 1].w};
-                storeGlobal32(reinterpret_cast<uint4*>(out) + i, u);
+            for (int j = 0; j < kWidth / 16; ++j) {
+                const uint4 w = outputPiece<T>(r + box * kPerBox + j * kPer16<T>, bias + 4 * (box * kPerBox + j * kPer16<T>));
+                const uint32_t piece = kWidth == 128 ? j ^ (lane & 7) : j;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                             ::"r"(at + lane * kWidth + piece * 16), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                             : "memory");
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16 / kE; ++i)
-                reinterpret_cast<uint4*>(out)[i] = w[i];
+            dev::fenceProxyAsyncShared();
+            __syncwarp();
+            if (lane == 0)
+                tmaStore2d(map, at, n0 + box * kPerBox, uint32_t(row0));
         }
-    } else {
+    } else if (row0 + lane < p.m) {
+        T* out = static_cast<T*>(p.out) + (row0 + lane) * p.outStride + n0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (c + i < p.n)
-                out[i] = fromFloat<T>(v[i]);
+        for (int i = 0; i < L::kHalf; ++i)
+            if (n0 + i < p.n)
+                out[i] = fromFloat<T>(__uint_as_float(r[i]) + __uint_as_float(dev::ldsU32(bias + 4 * i)));
     }
 }
 
-template <int BN, bool KN>
-__global__ void __launch_bounds__(Tile<BN, KN>::kThreads, 1)
-    productTiles(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const ProductArgs p) {
-    using L = Tile<BN, KN>;
+template <int BN, int CG, bool KN>
+__global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
+    productTiles(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+                 const __grid_constant__ CUtensorMap mapOut, const ProductArgs p) {
+    using L = Tile<BN, CG>;
     extern __shared__ unsigned char smemRaw[];
     const uint32_t base = (dev::smemAddr(smemRaw) + 1023u) & ~1023u;
     unsigned char* smem = smemRaw + (base - dev::smemAddr(smemRaw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full = base + L::kBarOff, empty = full + 8 * L::kStages;
-    const uint32_t scaleFull = empty + 8 * L::kStages, scaleEmpty = scaleFull + 8 * L::kSlots;
+    const uint32_t peerFull = empty + 8 * L::kStages; // in the first CTA: the second's stage and scales are there
+    const uint32_t scaleFull = peerFull + 8 * L::kStages, scaleEmpty = scaleFull + 8 * L::kSlots;
     const uint32_t accFull = scaleEmpty + 8 * L::kSlots, accEmpty = accFull + 8 * L::kAcc;
     const uint32_t tmemSlot = accEmpty + 8 * L::kAcc;
+    const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i)
-            dev::mbarInit(full + 8 * i, 1), dev::mbarInit(empty + 8 * i, 1);
+            dev::mbarInit(full + 8 * i, 1), dev::mbarInit(empty + 8 * i, 1), dev::mbarInit(peerFull + 8 * i, 1);
         for (int i = 0; i < L::kSlots; ++i)
             dev::mbarInit(scaleFull + 8 * i, 1), dev::mbarInit(scaleEmpty + 8 * i, 1);
         for (int i = 0; i < L::kAcc; ++i)
-            dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, L::kEpilogueWarps);
+            dev::mbarInit(accFull + 8 * i, 1), dev::mbarInit(accEmpty + 8 * i, L::kEpilogueWarps * CG);
         dev::fenceBarrierInit();
     }
-    if (warp == L::kMmaWarp) {
-        dev::tmemAlloc(tmemSlot, L::kTmemCols);
-        dev::tmemRelinquish();
-    }
+    if (warp == L::kMmaWarp)
+        tmemAllocGroup<CG>(tmemSlot, L::kTmemCols);
     dev::tcFenceBefore();
-    __syncthreads();
+    clusterSync<CG>();
     dev::tcFenceAfter();
     const uint32_t tmem = dev::ldsU32(tmemSlot);
     const uint32_t scaleTmem = tmem + L::kAcc * BN;
     const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, groups = (kBlocks + 3) / 4;
-    const uint32_t tiles = p.tilesM * p.tilesN;
+    const uint32_t tiles = p.tilesM * p.tilesN, firstTile = blockIdx.x / CG, tileStep = gridDim.x / CG;
 
     if (warp == L::kTmaWarp) {
         if (lane == 0) {
             tmaPrefetchMap(&mapA);
             tmaPrefetchMap(&mapB);
-            uint32_t it = 0;
+            uint32_t it = 0, stage = 0, phase = 1; // a stage's first turn does not wait
             bool ok = true;
-            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (uint32_t t = firstTile; t < tiles && ok; t += tileStep) {
                 uint64_t m0;
                 uint32_t n0;
-                tilePlace(p, t, m0, n0, BN);
+                tilePlace<L>(p, t, m0, n0);
+                m0 += 128 * rank, n0 += L::kBRows * rank;
                 for (uint32_t kb = 0; kb < kBlocks; ++kb, ++it) {
-                    const uint32_t s = it % L::kStages, turn = it / L::kStages;
-                    if (turn != 0 && !waitPhase(empty + 8 * s, (turn - 1) & 1)) {
+                    if (!waitPhase(empty + 8 * stage, phase)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t a = base + s * L::kStageBytes, b = a + L::kABytes;
-                    dev::mbarArriveExpectTx(full + 8 * s, L::kStageBytes);
-                    tmaLoad2d(a, &mapA, kb * kBlock, uint32_t(m0), full + 8 * s);
-                    if constexpr (KN) {
-#pragma unroll
-                        for (int j = 0; j < BN / 128; ++j)
-                            tmaLoad2d(b + j * 16384, &mapB, n0 + 128 * j, kb * kBlock, full + 8 * s);
-                    } else {
-                        tmaLoad2d(b, &mapB, kb * kBlock, n0, full + 8 * s);
-                    }
+                    const uint32_t a = base + stage * L::kStageBytes, b = a + L::kABytes, bar = full + 8 * stage;
+                    dev::mbarArriveExpectTx(bar, L::kStageBytes);
+                    tmaLoad2d(a, &mapA, kb * kBlock, uint32_t(m0), bar);
+                    if constexpr (KN)
+                        tmaLoad2d(b, &mapB, n0, kb * kBlock, bar);
+                    else
+                        tmaLoad2d(b, &mapB, kb * kBlock, n0, bar);
+                    if (++stage == L::kStages)
+                        stage = 0, phase ^= 1;
                 }
             }
             // After a wait that ran out, no copy may still be on its way when the CTA exits.
@@ -299,73 +325,91 @@ __global__ void __launch_bounds__(Tile<BN, KN>::kThreads, 1)
                     waitPhase(full + 8 * (i % L::kStages), (i / L::kStages) & 1);
         }
         __syncwarp();
-    } else if (warp == L::kMmaWarp) {
+    } else if (warp == L::kMmaWarp && rank == 0) {
         // The whole warp in uniform control flow; one elected lane issues.
         const uint32_t elected = electLane();
-        uint32_t stage = 0, phase = 0, slot = 0, slotPhase = 0, acc = 0, accPhase = 1; // an accumulator's first turn does not wait
+        uint32_t stage = 0, phase = 0, slot = 0, slotPhase = 0, acc = 0, accPhase = 1;
         bool ok = true;
-        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (uint32_t t = firstTile; t < tiles && ok; t += tileStep) {
             if (!waitPhase(accEmpty + 8 * acc, accPhase))
                 break;
             dev::tcFenceAfter();
             const uint32_t d = tmem + acc * BN;
             for (uint32_t kb = 0; kb < kBlocks; ++kb) {
                 const uint32_t sa = scaleTmem + slot * L::kScaleCols, sb = sa + 4, byte = kb & 3;
-                if (byte == 0) {
-                    if (!waitPhase(scaleFull + 8 * slot, slotPhase)) {
-                        ok = false;
-                        break;
-                    }
-                    dev::tcFenceAfter();
-                    const uint32_t slab = base + L::kScaleOff + slot * L::kSlabs * 512;
-#pragma unroll
-                    for (int i = 0; i < L::kSlabs; ++i)
-                        tcCopyScales<1>(elected, sa + 4 * i, slabDesc(slab + 512 * i));
+                if (byte == 0 && !waitPhase(scaleFull + 8 * slot, slotPhase)) {
+                    ok = false;
+                    break;
                 }
-                if (!waitPhase(full + 8 * stage, phase)) {
+                if (!waitPhase(full + 8 * stage, phase) || (CG == 2 && !waitPhase(peerFull + 8 * stage, phase))) {
                     ok = false;
                     break;
                 }
                 dev::tcFenceAfter();
+                if (byte == 0) {
+                    const uint32_t slab = base + L::kScaleOff + slot * L::kSlabs * 512;
+#pragma unroll
+                    for (int i = 0; i < L::kSlabs; ++i)
+                        tcCopyScales<CG>(elected, sa + 4 * i, slabDesc(slab + 512 * i));
+                }
                 const uint32_t a = base + stage * L::kStageBytes, b = a + L::kABytes;
-                const uint64_t descA = swizzledDesc(a, 16, 1024);
-                const uint64_t descB = KN ? swizzledDesc(b, 16384, 1024) : swizzledDesc(b, 16, 1024);
+                const uint64_t descA = swizzledDesc(a, 16, 1024), descB = swizzledDesc(b, 16, 1024);
                 const uint32_t idesc = p.idesc | (byte << 29) | (byte << 4);
                 if (p.k - kb * kBlock >= kBlock) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mmaScaled8<1>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb,
-                                      j != 0 ? 1u : uint32_t(kb != 0));
+                        mmaScaled8<CG>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb,
+                                       j != 0 ? 1u : uint32_t(kb != 0));
                 } else { // the last block ends inside
                     const uint32_t steps = (p.k - kb * kBlock + 31) / 32;
                     for (uint32_t j = 0; j < steps; ++j)
-                        mmaScaled8<1>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
+                        mmaScaled8<CG>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
                 }
-                commitCluster<1>(elected, empty + 8 * stage);
+                commitCluster<CG>(elected, empty + 8 * stage);
                 if (++stage == L::kStages)
                     stage = 0, phase ^= 1;
                 if (byte == 3 || kb + 1 == kBlocks) {
-                    commitCluster<1>(elected, scaleEmpty + 8 * slot);
+                    commitCluster<CG>(elected, scaleEmpty + 8 * slot);
                     if (++slot == L::kSlots)
                         slot = 0, slotPhase ^= 1;
                 }
             }
             if (ok)
-                commitCluster<1>(elected, accFull + 8 * acc);
+                commitCluster<CG>(elected, accFull + 8 * acc);
             if (++acc == L::kAcc)
                 acc = 0, accPhase ^= 1;
         }
+    } else if (warp == L::kMmaWarp) {
+        // The second CTA of a pair tells the first that its stages and scales are there.
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0, slot = 0, slotPhase = 0;
+            bool ok = true;
+            for (uint32_t t = firstTile; t < tiles && ok; t += tileStep)
+                for (uint32_t kb = 0; kb < kBlocks; ++kb) {
+                    if ((kb % 4 == 0 && !waitPhase(scaleFull + 8 * slot, slotPhase)) || !waitPhase(full + 8 * stage, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    arriveLeader<CG>(peerFull + 8 * stage);
+                    if (++stage == L::kStages)
+                        stage = 0, phase ^= 1;
+                    if ((kb % 4 == 3 || kb + 1 == kBlocks) && ++slot == L::kSlots)
+                        slot = 0, slotPhase ^= 1;
+                }
+        }
+        __syncwarp();
     } else if (warp == L::kScaleWarp) {
-        // Lane i holds rows i, i + 32, i + 64 and i + 96 of a slab, 16 bytes in shared memory.
+        // Lane i holds rows i, i + 32, i + 64 and i + 96 of a slab, 16 bytes in shared memory: A's 128
+        // rows of this CTA, all of B's.
         constexpr int kWords = 4 * L::kSlabs;
         uint32_t w[kWords];
         auto fetch = [&](uint32_t t, uint32_t g) {
             uint64_t m0;
             uint32_t n0;
-            tilePlace(p, t, m0, n0, BN);
+            tilePlace<L>(p, t, m0, n0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                w[c] = scaleWord(p.a, m0 + 32 * c + lane, g);
+                w[c] = scaleWord(p.a, m0 + 128 * rank + 32 * c + lane, g);
 #pragma unroll
             for (int c = 0; c < kWords - 4; ++c) {
                 if (32 * c >= BN)
@@ -376,90 +420,99 @@ __global__ void __launch_bounds__(Tile<BN, KN>::kThreads, 1)
                     w[4 + c] = scaleWord(p.b, n0 + 32 * c + lane, g);
             }
         };
-        uint32_t group = 0;
+        uint32_t slot = 0, phase = 1;
         bool ok = true;
-        if (blockIdx.x < tiles)
-            fetch(blockIdx.x, 0);
-        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-            for (uint32_t g = 0; g < groups; ++g, ++group) {
-                const uint32_t slot = group % L::kSlots, turn = group / L::kSlots;
-                uint32_t held[kWords];
-#pragma unroll
-                for (int i = 0; i < kWords; ++i)
-                    held[i] = w[i];
-                if (g + 1 < groups) // the next words' loads run under this group's wait
-                    fetch(t, g + 1);
-                else if (uint64_t(t) + gridDim.x < tiles)
-                    fetch(t + gridDim.x, 0);
-                if (turn != 0 && !waitPhase(scaleEmpty + 8 * slot, (turn - 1) & 1)) {
+        if (firstTile < tiles)
+            fetch(firstTile, 0);
+        for (uint32_t t = firstTile; t < tiles && ok; t += tileStep)
+            for (uint32_t g = 0; g < groups; ++g) {
+                if (!waitPhase(scaleEmpty + 8 * slot, phase)) {
                     ok = false;
                     break;
                 }
                 unsigned char* slab = smem + L::kScaleOff + slot * L::kSlabs * 512 + 16 * lane;
 #pragma unroll
                 for (int i = 0; i < L::kSlabs; ++i)
-                    *reinterpret_cast<uint4*>(slab + 512 * i) =
-                        make_uint4(held[4 * i], held[4 * i + 1], held[4 * i + 2], held[4 * i + 3]);
+                    *reinterpret_cast<uint4*>(slab + 512 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 dev::fenceProxyAsyncShared();
                 __syncwarp();
                 if (lane == 0)
                     dev::mbarArrive(scaleFull + 8 * slot);
+                if (++slot == L::kSlots)
+                    slot = 0, phase ^= 1;
+                // The next words are loaded behind the fence, which would wait for them.
+                if (g + 1 < groups)
+                    fetch(t, g + 1);
+                else if (uint64_t(t) + tileStep < tiles)
+                    fetch(t + tileStep, 0);
             }
     } else {
-        constexpr int kHalf = BN / 2; // columns per warp: two warps share a lane quarter
-        const uint32_t quarter = warp % 4, half = warp / 4;
-        uint32_t seq = 0;
-        for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, ++seq) {
-            const uint32_t acc = seq % L::kAcc;
-            if (!waitPhase(accFull + 8 * acc, (seq / L::kAcc) & 1))
-                break;
-            dev::tcFenceAfter();
+        const uint32_t quarter = warp % 4, half = warp / 4; // two warps share a lane quarter
+        const uint32_t buf = base + L::kOutOff + warp * L::kOutBufs * 4096;
+        const uint32_t bias = base + L::kBiasOff + warp * L::kHalf * 4;
+        uint32_t acc = 0, phase = 0, biasAt = 0xFFFFFFFFu;
+        for (uint32_t t = firstTile; t < tiles; t += tileStep) {
             uint64_t m0;
             uint32_t n0;
-            tilePlace(p, t, m0, n0, BN);
-            const uint32_t from = tmem + acc * BN + half * kHalf + (quarter << 21); // lanes in bits 16-31
-            uint32_t r[kHalf];
-            if constexpr (kHalf == 16) {
+            tilePlace<L>(p, t, m0, n0);
+            n0 += half * L::kHalf;
+            if (n0 != biasAt) { // the warp's columns of the bias, zero where there is none
+                __syncwarp();
+                for (uint32_t i = lane; i < uint32_t(L::kHalf); i += 32) {
+                    const float v = p.bias != nullptr && n0 + i < p.n ? __ldg(p.bias + n0 + i) : 0.0f;
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias + 4 * i), "f"(v) : "memory");
+                }
+                __syncwarp();
+                biasAt = n0;
+            }
+            if (!waitPhase(accFull + 8 * acc, phase))
+                break;
+            dev::tcFenceAfter();
+            const uint32_t from = tmem + acc * BN + half * L::kHalf + (quarter << 21); // lanes in bits 16-31
+            uint32_t r[L::kHalf];
+            if constexpr (L::kHalf == 16) {
                 dev::tcLoad32x32bx16(from, r);
             } else {
 #pragma unroll
-                for (int i = 0; i < kHalf / 32; ++i)
+                for (int i = 0; i < L::kHalf / 32; ++i)
                     tcLoad32x32bx32(from + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * i));
             }
             dev::tcWaitLd();
             dev::tcFenceBefore();
             __syncwarp();
             if (lane == 0)
-                dev::mbarArrive(accEmpty + 8 * acc);
-            const uint64_t row = m0 + 32 * quarter + lane;
-            if (row < p.m) {
-#pragma unroll
-                for (int i = 0; i < kHalf / 16; ++i) {
-                    const uint32_t c = n0 + half * kHalf + 16 * i;
-                    if (p.outType == TCC_BF16)
-                        storeColumns16<__nv_bfloat16>(p, row, c, r + 16 * i);
-                    else if (p.outType == TCC_F32)
-                        storeColumns16<float>(p, row, c, r + 16 * i);
-                    else
-                        storeColumns16<__half>(p, row, c, r + 16 * i);
-                }
+                arriveLeader<CG>(accEmpty + 8 * acc);
+            if (++acc == L::kAcc)
+                acc = 0, phase ^= 1;
+            const uint64_t row0 = m0 + 128 * rank + 32 * quarter;
+            if (row0 < p.m && n0 < p.n) {
+                if (p.outType == TCC_BF16)
+                    storeTile<L, __nv_bfloat16>(p, &mapOut, r, buf, bias, row0, n0, lane);
+                else if (p.outType == TCC_F32)
+                    storeTile<L, float>(p, &mapOut, r, buf, bias, row0, n0, lane);
+                else
+                    storeTile<L, __half>(p, &mapOut, r, buf, bias, row0, n0, lane);
             }
         }
+        if (lane == 0) // shared memory stays until the stores have read it
+            tmaStoreWaitRead<0>();
     }
+    __syncwarp();
     dev::tcFenceBefore();
-    __syncthreads();
+    clusterSync<CG>(); // no CTA of a pair leaves while the other may still arrive on its barriers
     dev::tcFenceAfter();
     if (warp == L::kMmaWarp)
-        dev::tmemDealloc(tmem, L::kTmemCols);
+        tmemDeallocGroup<CG>(tmem, L::kTmemCols);
 }
 
 ScaleView scaleView(const Operand& o, uint32_t rows, uint32_t width) {
     return {o.scales, rows, o.rowShift, width, width % 4 == 0 && alignedTo(o.scales, 4)};
 }
 
-template <int BN, bool KN> void launchTiles(const Product& p) {
-    using L = Tile<BN, KN>;
-    const uint32_t kBlocks = ceilDiv(p.k, kBlock);
+template <int BN, int CG, bool KN> void launchTiles(const Product& p) {
+    using L = Tile<BN, CG>;
+    static_assert(!KN || L::kBRows == 128, "rows of a [k, n] operand are copied 128 bytes at a time");
+    const uint32_t kBlocks = ceilDiv(p.k, kBlock), outBytes = typeBytes(p.outType);
     ProductArgs args{};
     args.a = scaleView(p.a, p.m, kBlocks);
     args.b = KN ? ScaleView{p.b.scales, p.k, 7, ceilDiv(p.n, kBlock), false} : scaleView(p.b, p.n, kBlocks);
@@ -467,21 +520,38 @@ template <int BN, bool KN> void launchTiles(const Product& p) {
     args.out = p.out;
     args.outStride = p.outStride;
     args.outType = p.outType;
-    const uint64_t rowBytes = p.outStride * typeBytes(p.outType);
-    args.outAlign = rowsAlignedTo(p.out, rowBytes, 32) ? 32 : rowsAlignedTo(p.out, rowBytes, 16) ? 16 : 0;
+    args.outTma = rowsAlignedTo(p.out, p.outStride * outBytes, 16) && p.outStride < (1ull << 38);
     args.m = p.m, args.n = p.n, args.k = p.k;
-    args.tilesM = ceilDiv(p.m, 128u);
+    args.tilesM = ceilDiv<uint32_t>(p.m, 128 * CG);
     args.tilesN = ceilDiv<uint32_t>(p.n, BN);
-    require(uint64_t(args.tilesM) * args.tilesN <= 0x7FFFFFFFull, "too many output tiles for one call");
-    args.idesc = scaledIdesc(p.a.type == TCC_E5M2, p.b.type == TCC_E5M2, KN, BN);
+    require(uint64_t(args.tilesM) * args.tilesN <= 0x3FFFFFFFull, "too many output tiles for one call");
+    args.idesc = scaledIdesc(p.a.type == TCC_E5M2, p.b.type == TCC_E5M2, KN, 128 * CG, BN);
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const CUtensorMap mapA = tensorMap2d(p.a.data, u8, 1, p.m, p.k, p.a.stride, 128, 128);
     const CUtensorMap mapB = KN ? tensorMap2d(p.b.data, u8, 1, p.k, p.n, p.b.stride, 128, 128)
-                                : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, BN, 128);
-    allowSharedMemory<productTiles<BN, KN>>(L::kBytes);
-    const uint32_t grid = std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors());
-    productTiles<BN, KN><<<grid, L::kThreads, L::kBytes, p.stream>>>(mapA, mapB, args);
-    checkCudaCall(cudaGetLastError());
+                                : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, L::kBRows, 128);
+    CUtensorMap mapOut{};
+    if (args.outTma) {
+        const uint32_t width = std::min<uint32_t>(128, L::kHalf * outBytes);
+        mapOut = tensorMap2d(p.out,
+                             p.outType == TCC_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                             : p.outType == TCC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             outBytes, p.m, p.n, p.outStride, 32, width / outBytes,
+                             width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+    allowSharedMemory<productTiles<BN, CG, KN>>(L::kBytes);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(CG * std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors() / CG));
+    config.blockDim = dim3(L::kThreads);
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = p.stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN>, mapA, mapB, mapOut, args));
 }
 
 void launchProduct(const Product& p) {
@@ -497,14 +567,14 @@ void launchProduct(const Product& p) {
         return;
     }
     const uint64_t rowTiles = ceilDiv(p.m, 128u), sms = multiprocessors();
-    if (rowTiles * ceilDiv(p.n, 256u) >= sms && p.n > 128)
-        p.kn ? launchTiles<256, true>(p) : launchTiles<256, false>(p);
+    if (p.n > 128 && ceilDiv(p.m, 256u) * uint64_t(ceilDiv(p.n, 256u)) * 2 >= sms)
+        p.kn ? launchTiles<256, 2, true>(p) : launchTiles<256, 2, false>(p);
     else if (p.kn || rowTiles * ceilDiv(p.n, 128u) >= sms)
-        p.kn ? launchTiles<128, true>(p) : launchTiles<128, false>(p);
+        p.kn ? launchTiles<128, 1, true>(p) : launchTiles<128, 1, false>(p);
     else if (rowTiles * ceilDiv(p.n, 64u) >= sms)
-        launchTiles<64, false>(p);
+        launchTiles<64, 1, false>(p);
     else
-        launchTiles<32, false>(p);
+        launchTiles<32, 1, false>(p);
 }
 
 } // namespace
