@@ -105,14 +105,14 @@ template <typename T> void launchGeneric(const Product& p) {
 // E8M0 scales are the blocks' own bytes: the hardware takes one scale per 32 elements of k, and a
 // block's four groups take the same one, so no scale is applied outside the tensor core and the sum
 // over all of k stays in one FP32 accumulator in tensor memory. Scales travel as words of four
-// consecutive blocks per row, loaded by a warp of their own, copied to tensor memory by the MMA thread
+// consecutive blocks per row, loaded by warps of their own, copied to tensor memory by the MMA thread
 // and picked by the byte selector of the instruction descriptor. Eight warps bring finished tiles into
 // registers, release the accumulator, and write them by TMA through 4 KB of shared memory each.
 template <int BN_, int CG_> struct Tile {
     static constexpr int BN = BN_, CG = CG_;
     static constexpr int kStages = BN == 256 ? 5 : BN == 128 ? 4 : 6;
     static constexpr int kAcc = BN == 256 ? 1 : 2;       // accumulators in tensor memory
-    static constexpr int kSlots = 4;                     // groups of four blocks' scales
+    static constexpr int kSlots = 6;                     // groups of four blocks' scales
     static constexpr int kSlabs = 1 + (BN + 127) / 128;  // of 512 bytes: A's rows, B's rows
     static constexpr int kBRows = BN / CG;               // rows of b in this CTA
     static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
@@ -132,7 +132,9 @@ template <int BN_, int CG_> struct Tile {
     static constexpr int kScaleCols = 4 * kSlabs;
     static constexpr int kTmemCols = 512;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
-    static constexpr int kThreads = 32 * 11;
+    static constexpr int kScaleWarps = BN == 256 ? 2 : 3; // 13 warps would leave the epilogue 128 registers
+    static constexpr int kThreads = 32 * (kScaleWarp + kScaleWarps);
+    static_assert(kSlots % kScaleWarps == 0, "a slot belongs to one scale warp");
     static_assert(kAcc * BN + kSlots * kScaleCols <= kTmemCols && kBytes <= 232448, "resources");
 };
 
@@ -224,7 +226,7 @@ template <int LEFT> __device__ __forceinline__ void tmaStoreWaitRead() {
 // that TMA cannot write go straight from the registers.
 template <typename L, typename T>
 __device__ __forceinline__ void storeTile(const ProductArgs& p, const CUtensorMap* map, const uint32_t (&r)[L::kHalf],
-                                          uint32_t buf, uint32_t bias, uint64_t row0, uint32_t n0, uint32_t lane) {
+                                          uint32_t buf, uint32_t& turn, uint32_t bias, uint64_t row0, uint32_t n0, uint32_t lane) {
     constexpr int kWidth = L::kHalf * int(sizeof(T)) < 128 ? L::kHalf * int(sizeof(T)) : 128;
     constexpr int kPerBox = kWidth / int(sizeof(T)), kBoxes = L::kHalf / kPerBox;
     if (p.outTma) {
@@ -232,8 +234,9 @@ __device__ __forceinline__ void storeTile(const ProductArgs& p, const CUtensorMa
         for (int box = 0; box < kBoxes; ++box) {
             if (n0 + box * kPerBox >= p.n)
                 break;
-            const uint32_t at = buf + box % L::kOutBufs * 4096;
-            if (lane == 0) // the box that was stored from here before has been read
+            const uint32_t at = buf + turn * 4096;
+            turn = turn + 1 == L::kOutBufs ? 0 : turn + 1;
+            if (lane == 0) // the box that was last stored from here, kOutBufs boxes ago, has been read
                 tmaStoreWaitRead<L::kOutBufs - 1>();
             __syncwarp();
 #pragma unroll
@@ -398,15 +401,21 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                 }
         }
         __syncwarp();
-    } else if (warp == L::kScaleWarp) {
+    } else if (warp >= L::kScaleWarp) {
         // Lane i holds rows i, i + 32, i + 64 and i + 96 of a slab, 16 bytes in shared memory: A's 128
         // rows of this CTA, all of B's.
+        // The warps take groups in turn: one warp's loads, whose latency under a full memory bus is 2.6
+        // us, set the pace of short products. A slot always belongs to the same warp (kSlots is a
+        // multiple of their number), so no warp can be two of its phases away from another.
         constexpr int kWords = 4 * L::kSlabs;
-        uint32_t w[kWords];
-        auto fetch = [&](uint32_t t, uint32_t g) {
+        const uint32_t first = warp - L::kScaleWarp;
+        const uint64_t total = firstTile < tiles ? uint64_t((tiles - firstTile - 1) / tileStep + 1) * groups : 0;
+        uint32_t slot = first, phase = 1;
+        for (uint64_t i = first; i < total; i += L::kScaleWarps) {
+            const uint32_t turn = uint32_t(i / groups), g = uint32_t(i - uint64_t(turn) * groups);
             uint64_t m0;
-            uint32_t n0;
-            tilePlace<L>(p, t, m0, n0);
+            uint32_t n0, w[kWords];
+            tilePlace<L>(p, firstTile + turn * tileStep, m0, n0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 w[c] = scaleWord(p.a, m0 + 128 * rank + 32 * c + lane, g);
@@ -419,38 +428,25 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                 else
                     w[4 + c] = scaleWord(p.b, n0 + 32 * c + lane, g);
             }
-        };
-        uint32_t slot = 0, phase = 1;
-        bool ok = true;
-        if (firstTile < tiles)
-            fetch(firstTile, 0);
-        for (uint32_t t = firstTile; t < tiles && ok; t += tileStep)
-            for (uint32_t g = 0; g < groups; ++g) {
-                if (!waitPhase(scaleEmpty + 8 * slot, phase)) {
-                    ok = false;
-                    break;
-                }
-                unsigned char* slab = smem + L::kScaleOff + slot * L::kSlabs * 512 + 16 * lane;
+            if (!waitPhase(scaleEmpty + 8 * slot, phase))
+                break;
+            unsigned char* slab = smem + L::kScaleOff + slot * L::kSlabs * 512 + 16 * lane;
 #pragma unroll
-                for (int i = 0; i < L::kSlabs; ++i)
-                    *reinterpret_cast<uint4*>(slab + 512 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                dev::fenceProxyAsyncShared();
-                __syncwarp();
-                if (lane == 0)
-                    dev::mbarArrive(scaleFull + 8 * slot);
-                if (++slot == L::kSlots)
-                    slot = 0, phase ^= 1;
-                // The next words are loaded behind the fence, which would wait for them.
-                if (g + 1 < groups)
-                    fetch(t, g + 1);
-                else if (uint64_t(t) + tileStep < tiles)
-                    fetch(t + tileStep, 0);
-            }
+            for (int j = 0; j < L::kSlabs; ++j)
+                *reinterpret_cast<uint4*>(slab + 512 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            dev::fenceProxyAsyncShared();
+            __syncwarp();
+            if (lane == 0)
+                dev::mbarArrive(scaleFull + 8 * slot);
+            slot += L::kScaleWarps;
+            if (slot >= L::kSlots)
+                slot = first, phase ^= 1;
+        }
     } else {
         const uint32_t quarter = warp % 4, half = warp / 4; // two warps share a lane quarter
         const uint32_t buf = base + L::kOutOff + warp * L::kOutBufs * 4096;
         const uint32_t bias = base + L::kBiasOff + warp * L::kHalf * 4;
-        uint32_t acc = 0, phase = 0, biasAt = 0xFFFFFFFFu;
+        uint32_t acc = 0, phase = 0, turn = 0, biasAt = 0xFFFFFFFFu;
         for (uint32_t t = firstTile; t < tiles; t += tileStep) {
             uint64_t m0;
             uint32_t n0;
@@ -487,11 +483,11 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
             const uint64_t row0 = m0 + 128 * rank + 32 * quarter;
             if (row0 < p.m && n0 < p.n) {
                 if (p.outType == TCC_BF16)
-                    storeTile<L, __nv_bfloat16>(p, &mapOut, r, buf, bias, row0, n0, lane);
+                    storeTile<L, __nv_bfloat16>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
                 else if (p.outType == TCC_F32)
-                    storeTile<L, float>(p, &mapOut, r, buf, bias, row0, n0, lane);
+                    storeTile<L, float>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
                 else
-                    storeTile<L, __half>(p, &mapOut, r, buf, bias, row0, n0, lane);
+                    storeTile<L, __half>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
             }
         }
         if (lane == 0) // shared memory stays until the stores have read it
