@@ -140,6 +140,10 @@ SIGNATURES = {
                                        C.c_void_p]),
 }
 
+# The dense operators with their arguments as an array of 64-bit words (exported for dense.py, not
+# declared in the public header).
+PACKED_SIGNATURES = {"tcc_dense8_call": (C.c_int, [C.c_int, C.c_char_p])}
+
 # Failure-path test hooks of the library (exported, not declared in the public header).
 TEST_SIGNATURES = {
     "tcc_test_launch_spmm_int8_stalled": (C.c_int, [C.POINTER(Sw32DeviceView), C.c_void_p, C.c_void_p, C.c_void_p,
@@ -187,7 +191,7 @@ def _load(path: Path, signatures: dict) -> C.CDLL:
 def lib() -> C.CDLL:
     global _lib
     if _lib is None:
-        _lib = _load(library_path(), {**SIGNATURES, **TEST_SIGNATURES})
+        _lib = _load(library_path(), {**SIGNATURES, **PACKED_SIGNATURES, **TEST_SIGNATURES})
     return _lib
 
 

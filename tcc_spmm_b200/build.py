@@ -26,7 +26,8 @@ CUDA_INCLUDE = Path(NVCC).resolve().parent.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 LIB_SOURCES = ["format.cpp", "capi_host.cpp", "cxx_api.cpp", "upload.cpp", "features.cu", "spmm.cu", "format_gpu.cu",
-               "matrix_market.cpp", "blocks8.cu", "matmul_fp8.cu", "weight_grad.cu"]
+               "matrix_market.cpp", "blocks8.cu", "matmul_fp8.cu", "weight_grad.cu",
+               "dense8_call.cpp"]
 
 
 def _run(cmd: list[str]) -> None:

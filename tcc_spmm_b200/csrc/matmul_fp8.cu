@@ -98,6 +98,160 @@ template <typename T> void launchGeneric(const Product& p) {
     checkCudaCall(cudaGetLastError());
 }
 
+// ---- few rows of a ------------------------------------------------------------------------------
+// With up to 16 rows of a the product is a read of b. A CTA takes 16 rows of b; its warps take blocks of
+// 128 of k in turn, each with a ring of its own of asynchronous copies (no barrier between warps, and
+// all of a 4096-wide row in flight at once), and their sums are added up in shared memory at the end, in
+// a fixed order. The order of k in mma.m16n8k32 may be any that both operands share, so a lane reads 16
+// bytes of k of two rows of b and of MT rows of a at a time: two MMAs per 64 of k and 8 rows of a. The sum
+// over a block is multiplied by the two scales' product, a power of two.
+template <int MT_> struct Few {
+    static constexpr int MT = MT_;
+    static constexpr int kWarps = 8, kRows = 16;         // rows of b per CTA
+    static constexpr int kStages = MT == 1 ? 4 : 3;
+    static constexpr int kStageBytes = (kRows + 8 * MT) * 128;
+    static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+    static constexpr uint32_t kMostBlocks = 512;         // blocks of k whose scales fit beside the rings
+    static int bytes(uint32_t kBlocks) { return kRingBytes + int(kRows + 8 * MT) * int(kBlocks); }
+};
+
+// Rows of 8-bit floats from the row-major operand; which is which in mma.m16n8k32 follows the types.
+template <bool TA5, bool TB5>
+__device__ __forceinline__ void mmaFp8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+#define TCC_MMA(TA, TB)                                                                                             \
+    asm("mma.sync.aligned.m16n8k32.row.col.f32." TA "." TB ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                            \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+    if constexpr (TA5 && TB5)
+        TCC_MMA("e5m2", "e5m2");
+    else if constexpr (TA5)
+        TCC_MMA("e5m2", "e4m3");
+    else if constexpr (TB5)
+        TCC_MMA("e4m3", "e5m2");
+    else
+        TCC_MMA("e4m3", "e4m3");
+#undef TCC_MMA
+}
+// 16 bytes to shared memory, the last 16 - bytes of them zero.
+__device__ __forceinline__ void cpAsync16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int MT, bool A5, bool B5, typename T>
+__global__ void __launch_bounds__(32 * Few<MT>::kWarps)
+    productFew(const Operand a, const Operand b, const float* __restrict__ bias, T* __restrict__ out, uint64_t outStride,
+               uint32_t m, uint32_t n, uint32_t k) {
+    using L = Few<MT>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const uint64_t n0 = uint64_t(blockIdx.x) * L::kRows;
+    const uint32_t kBlocks = (k + kBlock - 1) / kBlock;
+    const uint32_t ring = dev::smemAddr(smem) + warp * L::kStages * L::kStageBytes;
+    // Copies of a block: a lane's 16-byte piece of rows lane / 8, + 4, ... Rows outside copy the last row
+    // instead: their sums go nowhere. Odd rows swap their 64-byte halves, for the banks.
+    const uint32_t piece = lane % 8, row0 = lane / 8;
+    auto copy = [&](uint32_t kb, uint32_t stage) {
+        const uint32_t to = ring + stage * L::kStageBytes + ((piece ^ ((row0 & 1) << 2)) * 16) + row0 * 128;
+        const uint32_t c = kb * kBlock + 16 * piece;
+        const uint32_t bytes = c < k ? min(16u, k - c) : 0u, at = c < k ? c : 0u;
+#pragma unroll
+        for (int i = 0; i < L::kRows / 4; ++i)
+            cpAsync16(to + 512 * i, b.data + min(n0 + row0 + 4 * i, uint64_t(n - 1)) * b.stride + at, bytes);
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
+            cpAsync16(to + L::kRows * 128 + 512 * i, a.data + uint64_t(min(row0 + 4 * i, m - 1)) * a.stride + at, bytes);
+    };
+#pragma unroll
+    for (int i = 0; i < L::kStages; ++i) {
+        if (warp + i * L::kWarps < kBlocks)
+            copy(warp + i * L::kWarps, i);
+        dev::cpAsyncCommit();
+    }
+    // Scale bytes of the CTA's rows of b, then of a: [row][block].
+    unsigned char* scales = smem + L::kRingBytes;
+    for (uint32_t i = threadIdx.x; i < (L::kRows + 8 * MT) * kBlocks; i += 32 * L::kWarps) {
+        const uint32_t row = i / kBlocks, kb = i - row * kBlocks;
+        scales[i] = row < L::kRows ? __ldg(b.scales + (min(n0 + row, uint64_t(n - 1)) >> b.rowShift) * kBlocks + kb)
+                                   : __ldg(a.scales + uint64_t(min(row - L::kRows, m - 1) >> a.rowShift) * kBlocks + kb);
+    }
+    __syncthreads();
+    float acc[MT][4] = {};
+    uint32_t stage = 0;
+    for (uint32_t kb = warp; kb < kBlocks; kb += L::kWarps) {
+        dev::cpAsyncWaitGroup<L::kStages - 1>();
+        __syncwarp();
+        const uint32_t from = ring + stage * L::kStageBytes + g * 128;
+        float part[MT][4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t at = from + (((4 * h + t) ^ ((g & 1) << 2)) * 16);
+            const uint4 u = dev::ldsV4(at), v = dev::ldsV4(at + 1024);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const uint4 x = dev::ldsV4(at + L::kRows * 128 + 1024 * j);
+                mmaFp8<B5, A5>(part[j], u.x, v.x, u.y, v.y, x.x, x.y);
+                mmaFp8<B5, A5>(part[j], u.z, v.z, u.w, v.w, x.z, x.w);
+            }
+        }
+        const float sb[2] = {scaleValue(scales[g * kBlocks + kb]), scaleValue(scales[(g + 8) * kBlocks + kb])};
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const unsigned char* sa = scales + (L::kRows + 8 * j + 2 * t) * kBlocks + kb;
+            const float s0 = scaleValue(sa[0]), s1 = scaleValue(sa[kBlocks]);
+            acc[j][0] = fmaf(part[j][0], sb[0] * s0, acc[j][0]);
+            acc[j][1] = fmaf(part[j][1], sb[0] * s1, acc[j][1]);
+            acc[j][2] = fmaf(part[j][2], sb[1] * s0, acc[j][2]);
+            acc[j][3] = fmaf(part[j][3], sb[1] * s1, acc[j][3]);
+        }
+        __syncwarp(); // every lane has read the stage
+        if (kb + L::kStages * L::kWarps < kBlocks)
+            copy(kb + L::kStages * L::kWarps, stage);
+        dev::cpAsyncCommit();
+        stage = stage + 1 == L::kStages ? 0 : stage + 1;
+    }
+    dev::cpAsyncWaitAll();
+    __syncthreads(); // the rings become the sums
+    float(*sums)[L::kRows][8 * MT + 1] = reinterpret_cast<float(*)[L::kRows][8 * MT + 1]>(smem);
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            sums[warp][g + 8 * (i / 2)][8 * j + 2 * t + i % 2] = acc[j][i];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < L::kRows * 8 * MT; i += 32 * L::kWarps) {
+        const uint32_t row = i / L::kRows, c = i % L::kRows; // row of a, row of b within the CTA's
+        if (row < m && n0 + c < n) {
+            float sum = bias ? bias[n0 + c] : 0.0f;
+#pragma unroll
+            for (int w = 0; w < L::kWarps; ++w)
+                sum += sums[w][c][row];
+            out[row * outStride + n0 + c] = fromFloat<T>(sum);
+        }
+    }
+}
+
+template <int MT, bool A5, bool B5, typename T> void launchFewTo(const Product& p) {
+    using L = Few<MT>;
+    allowSharedMemory<productFew<MT, A5, B5, T>>(L::bytes(L::kMostBlocks));
+    productFew<MT, A5, B5, T><<<ceilDiv<uint32_t>(p.n, L::kRows), 32 * L::kWarps, L::bytes(ceilDiv(p.k, kBlock)), p.stream>>>(
+        p.a, p.b, p.bias, static_cast<T*>(p.out), p.outStride, p.m, p.n, p.k);
+    checkCudaCall(cudaGetLastError());
+}
+template <int MT, bool A5, bool B5> void launchFewTyped(const Product& p) {
+    switch (p.outType) {
+    case TCC_F32: launchFewTo<MT, A5, B5, float>(p); break;
+    case TCC_BF16: launchFewTo<MT, A5, B5, __nv_bfloat16>(p); break;
+    default: launchFewTo<MT, A5, B5, __half>(p); break;
+    }
+}
+template <int MT> void launchFew(const Product& p) {
+    if (p.a.type == TCC_E5M2)
+        p.b.type == TCC_E5M2 ? launchFewTyped<MT, true, true>(p) : launchFewTyped<MT, true, false>(p);
+    else
+        p.b.type == TCC_E5M2 ? launchFewTyped<MT, false, true>(p) : launchFewTyped<MT, false, false>(p);
+}
+
 // ---- tensor cores -------------------------------------------------------------------------------
 // Persistent clusters of CG CTAs (one per SM) compute tiles of 128 CG x BN outputs. A warp issues TMA
 // copies of 128 bytes of k per stage (128-byte swizzle); one thread issues tcgen05.mma kind::mxf8f6f4,
@@ -560,6 +714,10 @@ void launchProduct(const Product& p) {
         case TCC_BF16: launchGeneric<__nv_bfloat16>(p); break;
         default: launchGeneric<__half>(p); break;
         }
+        return;
+    }
+    if (p.m <= 16 && !p.kn && ceilDiv(p.k, kBlock) <= Few<1>::kMostBlocks) {
+        p.m <= 8 ? launchFew<1>(p) : launchFew<2>(p);
         return;
     }
     const uint64_t rowTiles = ceilDiv(p.m, 128u), sms = multiprocessors();

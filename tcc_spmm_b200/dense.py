@@ -11,11 +11,13 @@ device), never synchronise, and raise InvalidArgument for tensors that do not fi
 write into tensors that the caller gives. The reference has no counterpart.
 
 The checks run on every call, and a small operator takes a few microseconds, so they are written
-for speed: plain comparisons, with messages formed only when one fails.
+for speed: plain comparisons, with messages formed only when one fails, and one packed argument
+for the library.
 """
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 from . import _native as N
@@ -25,65 +27,75 @@ BLOCK = 128
 ACTIVATIONS = {"relu": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "identity": 4}
 LAYOUTS = {"nk": 0, "kn": 1}
 
-_torch = None     # torch, its raw-stream and device queries, and the type codes, once used
+# torch, its raw-stream and current-device queries, and the type codes, once an operator is used
+_torch = _raw_stream = _current_device = _call = None
 _TYPES: dict = {}
-_FLOATS, _FP8 = frozenset((0, 1, 2)), frozenset((3, 4))
+_SCALES: set = set()
+_FLOATS, _FP8 = (0, 1, 2), (3, 4)
 
 
 def _load():
-    global _torch
+    global _torch, _raw_stream, _current_device, _call
     import torch
 
     _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
                    torch.float8_e5m2: 4})
+    _SCALES.update((torch.uint8, torch.float8_e8m0fnu))
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _call = N.lib().tcc_dense8_call
     _torch = torch
-    return torch
 
 
 def _refuse(message: str):
     raise InvalidArgument(message)
 
 
-def _matrix(name: str, t, device=None, shape=None) -> int:
-    """Checks a 2-D operand and returns its row stride in elements."""
-    torch = _torch or _load()
-    if not isinstance(t, torch.Tensor) or t.dim() != 2:
-        _refuse(f"{name} must be a 2-D tensor")
-    if not t.is_cuda:
+def _matrix(name: str, t, device: int = -1) -> tuple:
+    """(rows, columns, row stride in elements, device) of a 2-D CUDA operand, on `device` if that is given."""
+    try:
+        rows, cols = t.shape
+        row_stride, col_stride = t.stride()
+        on = t.get_device()
+    except (AttributeError, TypeError, ValueError, RuntimeError):
+        _refuse(f"{name} must be a 2-D CUDA tensor")
+    if on < 0:
         _refuse(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        _refuse(f"{name} is on {t.device}, expected {device}")
-    rows, cols = t.shape
-    if shape is not None and (rows != shape[0] or cols != shape[1]):
-        _refuse(f"{name} has shape {(rows, cols)}, expected {tuple(shape)}")
-    if rows >= 2 ** 32 or cols >= 2 ** 32:
+    if on != device and device >= 0:
+        _refuse(f"{name} is on cuda:{on}, expected cuda:{device}")
+    if rows > 0xFFFFFFFF or cols > 0xFFFFFFFF:
         _refuse(f"{name} is too large")
-    row_stride, col_stride = t.stride()
-    if cols > 1 and col_stride != 1:
+    if col_stride != 1 and cols > 1:
         _refuse(f"{name} must have stride 1 along its last dimension")
     if rows <= 1:  # no second row: the distance to it says nothing
-        return -(-cols // 16) * 16
+        return rows, cols, (cols + 15) & -16, on
     if row_stride < cols:
         _refuse(f"the rows of {name} overlap")
-    return row_stride
+    return rows, cols, row_stride, on
 
 
-def _scales(name: str, t, device, rows: int, cols: int, row_blocks: bool = True, square_blocks: bool = True) -> int:
+def _shaped(name: str, t, rows: int, cols: int, device: int) -> int:
+    """The row stride of a 2-D CUDA operand that must have this shape."""
+    r, c, stride, _ = _matrix(name, t, device)
+    if r != rows or c != cols:
+        _refuse(f"{name} has shape {(r, c)}, expected {(rows, cols)}")
+    return stride
+
+
+def _scales(name: str, t, device: int, rows: int, cols: int, row_blocks: bool = True, square_blocks: bool = True) -> int:
     """Checks the scale bytes of a [rows, cols] matrix and returns the rows per block."""
-    torch = _torch
-    if not isinstance(t, torch.Tensor) or (t.dtype != torch.uint8 and t.dtype != torch.float8_e8m0fnu):
+    if t.dtype not in _SCALES:
         _refuse(f"{name} must hold scale bytes (uint8 or float8_e8m0fnu)")
-    if t.device != device:
-        _refuse(f"{name} is on {t.device}, expected {device}")
-    if t.dim() == 2 and t.is_contiguous():
-        r, c = t.shape
-        if c == -(-cols // BLOCK):
-            if row_blocks and r == rows:
-                return 1
-            if square_blocks and r == -(-rows // BLOCK):
-                return BLOCK
-    want = [(rows, -(-cols // BLOCK))] * row_blocks + [(-(-rows // BLOCK), -(-cols // BLOCK))] * square_blocks
-    _refuse(f"{name} has shape {tuple(t.shape)}, expected contiguous {' or '.join(map(str, want))}")
+    if t.get_device() != device:
+        _refuse(f"{name} is on {t.device}, expected cuda:{device}")
+    wide = (cols + 127) >> 7
+    shape = tuple(t.shape)
+    if t.is_contiguous():
+        if row_blocks and shape == (rows, wide):
+            return 1
+        if square_blocks and shape == ((rows + 127) >> 7, wide):
+            return BLOCK
+    want = [(rows, wide)] * row_blocks + [((rows + 127) >> 7, wide)] * square_blocks
+    _refuse(f"{name} has shape {shape}, expected contiguous {' or '.join(map(str, want))}")
 
 
 def _type(name: str, t, allowed) -> int:
@@ -93,16 +105,19 @@ def _type(name: str, t, allowed) -> int:
     return code
 
 
-def _launch(device, stream, call, *args) -> None:
-    """call(*args, stream) with `device` current."""
-    torch = _torch
-    index = device.index
-    raw = torch._C._cuda_getCurrentRawStream(index) if stream is None else _stream_handle(stream)
-    if index == torch._C._cuda_getDevice():
-        status = call(*args, raw)
+_QUANTIZE, _PRODUCT, _CHECKPOINT, _BACKWARD, _WEIGHT_GRAD = range(5)  # tcc_dense8_call's operators
+_words = [struct.Struct(f"{n}Q").pack for n in (11, 19, 12, 12, 15)]
+
+
+def _launch(device: int, stream, op: int, *args) -> None:
+    """Operator `op` with these arguments and the stream, with `device` current."""
+    raw = _raw_stream(device) if stream is None else _stream_handle(stream)
+    words = _words[op](*args, raw)
+    if device == _current_device():
+        status = _call(op, words)
     else:
-        with torch.cuda.device(device):
-            status = call(*args, raw)
+        with _torch.cuda.device(device):
+            status = _call(op, words)
     if status:
         _check(status)
 
@@ -113,15 +128,15 @@ def quantize_blocks_fp8(x, q, scales, block_rows: int = 1, stream=None) -> None:
     q: [rows, cols] of float8_e4m3fn or float8_e5m2; scales: [ceil(rows / block_rows),
     ceil(cols / 128)] bytes; block_rows 1 (activations) or 128 (weights). matmul_fp8_blocks runs
     fastest on a q whose rows start on 16 bytes."""
-    xs = _matrix("x", x)
-    device, shape = x.device, x.shape
-    qs = _matrix("q", q, device, shape)
+    if _torch is None:
+        _load()
+    rows, cols, xs, device = _matrix("x", x)
+    qs = _shaped("q", q, rows, cols, device)
     xt, qt = _type("x", x, _FLOATS), _type("q", q, _FP8)
     if block_rows != 1 and block_rows != BLOCK:
         _refuse("block_rows must be 1 or 128")
-    rows, cols = shape
     _scales("scales", scales, device, rows, cols, block_rows == 1, block_rows == BLOCK)
-    _launch(device, stream, N.lib().tcc_quantize_blocks_fp8, x.data_ptr(), xt, xs, q.data_ptr(), qt, qs,
+    _launch(device, stream, _QUANTIZE, x.data_ptr(), xt, xs, q.data_ptr(), qt, qs,
             scales.data_ptr(), rows, cols, block_rows)
 
 
@@ -133,25 +148,25 @@ def matmul_fp8_blocks(a, a_scales, b, b_scales, output, bias=None, b_layout: str
     a and b: float8_e4m3fn or float8_e5m2 blocks; the shapes of the scales tell blocks of a row from
     blocks of 128 x 128 (b [k, n] needs the latter). The sum is accumulated in fp32 and rounded once
     to output's type (fp32, bf16 or fp16)."""
+    if _torch is None:
+        _load()
     layout = LAYOUTS.get(b_layout)
     if layout is None:
         _refuse(f"b_layout must be one of {sorted(LAYOUTS)}")
-    as_ = _matrix("a", a)
-    device, (m, k) = a.device, a.shape
-    bs = _matrix("b", b, device)
-    b_rows, b_cols = b.shape
+    m, k, as_, device = _matrix("a", a)
+    b_rows, b_cols, bs, _ = _matrix("b", b, device)
     n, b_k = (b_cols, b_rows) if layout else (b_rows, b_cols)
     if b_k != k:
         _refuse(f"b has shape {(b_rows, b_cols)} in layout {b_layout}, but k is {k}")
-    os_ = _matrix("output", output, device, (m, n))
+    os_ = _shaped("output", output, m, n, device)
     at, bt, ot = _type("a", a, _FP8), _type("b", b, _FP8), _type("output", output, _FLOATS)
     a_block = _scales("a_scales", a_scales, device, m, k)
     b_block = _scales("b_scales", b_scales, device, b_rows, b_cols, not layout)
-    if bias is not None and not (bias.dtype == _torch.float32 and bias.dim() == 1 and bias.numel() == n and
-                                 bias.is_contiguous() and bias.device == device):
-        _refuse(f"bias must be {n} contiguous fp32 values on {device}")
-    _launch(device, stream, N.lib().tcc_matmul_fp8_blocks, a.data_ptr(), at, as_, a_scales.data_ptr(), a_block,
-            b.data_ptr(), bt, bs, b_scales.data_ptr(), b_block, layout, None if bias is None else bias.data_ptr(),
+    if bias is not None and not (bias.dtype == _torch.float32 and tuple(bias.shape) == (n,) and bias.is_contiguous() and
+                                 bias.get_device() == device):
+        _refuse(f"bias must be {n} contiguous fp32 values on cuda:{device}")
+    _launch(device, stream, _PRODUCT, a.data_ptr(), at, as_, a_scales.data_ptr(), a_block,
+            b.data_ptr(), bt, bs, b_scales.data_ptr(), b_block, layout, 0 if bias is None else bias.data_ptr(),
             output.data_ptr(), ot, os_, m, n, k)
 
 
@@ -174,24 +189,24 @@ def activation_checkpoint_int8(x, y, q, scales, activation: str = "gelu", stream
     x, y: [rows, cols] of one type (fp32, bf16 or fp16), y may be x itself; q: int8 [rows, cols];
     scales: [rows, ceil(cols / 128)] bytes. activation: relu, gelu, gelu_tanh, silu, or identity,
     which keeps x alone (y None)."""
+    if _torch is None:
+        _load()
     code = ACTIVATIONS.get(activation)
     if code is None:
         _refuse(f"activation must be one of {sorted(ACTIVATIONS)}")
-    xs = _matrix("x", x)
-    device, shape = x.device, x.shape
+    rows, cols, xs, device = _matrix("x", x)
     xt = _type("x", x, _FLOATS)
     if activation == "identity":
         if y is not None:
             _refuse("the identity writes no y: pass None")
-        ys, y_ptr = 0, None
+        ys = y_ptr = 0
     else:
-        ys, y_ptr = _matrix("y", y, device, shape), y.data_ptr()
+        ys, y_ptr = _shaped("y", y, rows, cols, device), y.data_ptr()
         _pair("y", y, x, ys, xs)
-    qs = _matrix("q", q, device, shape)
+    qs = _shaped("q", q, rows, cols, device)
     _int8("q", q)
-    rows, cols = shape
     _scales("scales", scales, device, rows, cols, True, False)
-    _launch(device, stream, N.lib().tcc_activation_checkpoint_int8, x.data_ptr(), xs, y_ptr, ys, xt, q.data_ptr(), qs,
+    _launch(device, stream, _CHECKPOINT, x.data_ptr(), xs, y_ptr, ys, xt, q.data_ptr(), qs,
             scales.data_ptr(), rows, cols, code)
 
 
@@ -201,19 +216,19 @@ def activation_backward_int8(grad_y, q, scales, grad_x, activation: str = "gelu"
 
     grad_y, grad_x: [rows, cols] of one type (fp32, bf16 or fp16); grad_x may be grad_y itself.
     ReLU passes the gradient where x^ > 0."""
+    if _torch is None:
+        _load()
     code = ACTIVATIONS.get(activation)
     if code is None or activation == "identity":
         _refuse(f"activation must be one of {sorted(set(ACTIVATIONS) - {'identity'})}")
-    gs = _matrix("grad_y", grad_y)
-    device, shape = grad_y.device, grad_y.shape
+    rows, cols, gs, device = _matrix("grad_y", grad_y)
     gt = _type("grad_y", grad_y, _FLOATS)
-    xs = _matrix("grad_x", grad_x, device, shape)
+    xs = _shaped("grad_x", grad_x, rows, cols, device)
     _pair("grad_x", grad_x, grad_y, xs, gs)
-    qs = _matrix("q", q, device, shape)
+    qs = _shaped("q", q, rows, cols, device)
     _int8("q", q)
-    rows, cols = shape
     _scales("scales", scales, device, rows, cols, True, False)
-    _launch(device, stream, N.lib().tcc_activation_backward_int8, grad_y.data_ptr(), gs, gt, q.data_ptr(), qs,
+    _launch(device, stream, _BACKWARD, grad_y.data_ptr(), gs, gt, q.data_ptr(), qs,
             scales.data_ptr(), grad_x.data_ptr(), xs, rows, cols, code)
 
 
@@ -233,29 +248,29 @@ def weight_grad_int8(grad_y, q, scales, grad_w, accumulate: bool = False, worksp
     grad_y: fp32, bf16 or fp16; grad_w: fp32. workspace: a contiguous CUDA tensor of
     weight_grad_int8_workspace_size bytes or more, not shared with a call that may run at the same
     time; None takes it from torch's allocator, on the stream of the call."""
-    gs = _matrix("grad_y", grad_y)
-    torch = _torch
-    device, (rows, n) = grad_y.device, grad_y.shape
+    if _torch is None:
+        _load()
+    rows, n, gs, device = _matrix("grad_y", grad_y)
     gt = _type("grad_y", grad_y, _FLOATS)
-    qs = _matrix("q", q, device)
-    q_rows, k = q.shape
+    q_rows, k, qs, _ = _matrix("q", q, device)
     if q_rows != rows:
         _refuse(f"q has {q_rows} rows, grad_y {rows}")
     _int8("q", q)
-    ws = _matrix("grad_w", grad_w, device, (n, k))
-    if grad_w.dtype != torch.float32:
+    ws = _shaped("grad_w", grad_w, n, k, device)
+    if grad_w.dtype != _torch.float32:
         _refuse("grad_w must be fp32")
     _scales("scales", scales, device, rows, k, True, False)
     if workspace is None:
         need = weight_grad_int8_workspace_size(rows, n, k)
         if need:
             if isinstance(stream, int):
-                stream = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
-            with torch.cuda.stream(stream):  # nothing for None: the current stream
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
-        _refuse(f"the workspace must be contiguous on {device}")
+                cuda = _torch.cuda
+                stream = cuda.ExternalStream(stream, device) if stream else cuda.default_stream(device)
+            with _torch.cuda.stream(stream):  # nothing for None: the current stream
+                workspace = _torch.empty(need, dtype=_torch.uint8, device=grad_y.device)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        _refuse(f"the workspace must be contiguous on cuda:{device}")
     have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _launch(device, stream, N.lib().tcc_weight_grad_int8, grad_y.data_ptr(), gt, gs, q.data_ptr(), qs,
+    _launch(device, stream, _WEIGHT_GRAD, grad_y.data_ptr(), gt, gs, q.data_ptr(), qs,
             scales.data_ptr(), grad_w.data_ptr(), ws, rows, n, k, 1 if accumulate else 0,
-            None if workspace is None else workspace.data_ptr(), have)
+            0 if workspace is None else workspace.data_ptr(), have)
