@@ -42,6 +42,29 @@ __device__ __forceinline__ Place placeOf(uint64_t blocks, uint32_t colBlocks) {
     return p;
 }
 
+// 16 bytes from or to an address that is `align` bytes aligned (16, 8 or 4; the same in every thread).
+__device__ __forceinline__ uint4 loadWords16(const void* p, uint32_t align) {
+    if (align >= 16)
+        return __ldcs(reinterpret_cast<const uint4*>(p));
+    if (align == 8) {
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p)), b = __ldcs(reinterpret_cast<const uint2*>(p) + 1);
+        return make_uint4(a.x, a.y, b.x, b.y);
+    }
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+    return make_uint4(__ldcs(w), __ldcs(w + 1), __ldcs(w + 2), __ldcs(w + 3));
+}
+__device__ __forceinline__ void storeWords16(void* p, uint4 v, uint32_t align) {
+    if (align >= 16) {
+        __stcs(reinterpret_cast<uint4*>(p), v);
+    } else if (align == 8) {
+        __stcs(reinterpret_cast<uint2*>(p), make_uint2(v.x, v.y));
+        __stcs(reinterpret_cast<uint2*>(p) + 1, make_uint2(v.z, v.w));
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(p);
+        __stcs(w, v.x), __stcs(w + 1, v.y), __stcs(w + 2, v.z), __stcs(w + 3, v.w);
+    }
+}
+
 // One lane's share of a block of x: pieces of 16 bytes (kPer16 elements), piece i at column
 // kPer16 * (8 i + lane), as they were loaded. Columns at or beyond `left` read as zero.
 template <typename T> struct Share {
@@ -49,8 +72,8 @@ template <typename T> struct Share {
     static constexpr int kPieces = kBlock / kGroup / kElems;
     uint4 raw[kPieces];
     static __device__ __forceinline__ uint32_t column(int i, uint32_t lane) { return kElems * (kGroup * i + lane); }
-    __device__ __forceinline__ void load(const T* row, uint32_t left, uint32_t lane, bool vector) {
-        if (vector && left >= kBlock) {
+    __device__ __forceinline__ void load(const T* row, uint32_t left, uint32_t lane, uint32_t align) {
+        if (align >= 16 && left >= kBlock) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
                 raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + column(i, lane)));
@@ -59,8 +82,8 @@ template <typename T> struct Share {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const uint32_t c = column(i, lane);
-            if (vector && c + kElems <= left) {
-                raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + c));
+            if (align >= 4 && c + kElems <= left) {
+                raw[i] = loadWords16(row + c, align);
             } else {
                 float v[kElems];
 #pragma unroll
@@ -72,10 +95,10 @@ template <typename T> struct Share {
     }
     // Piece i of a row of T.
     static __device__ __forceinline__ void store(T* row, int i, const float (&v)[kElems], uint32_t left, uint32_t lane,
-                                                 bool vector) {
+                                                 uint32_t align) {
         const uint32_t c = column(i, lane);
-        if (vector && c + kElems <= left) {
-            __stcs(reinterpret_cast<uint4*>(row + c), pack16<T>(v));
+        if (align >= 4 && c + kElems <= left) {
+            storeWords16(row + c, pack16<T>(v), align);
         } else {
 #pragma unroll
             for (int e = 0; e < kElems; ++e)
@@ -105,13 +128,13 @@ __device__ __forceinline__ void storeBytes(uint8_t* q, const uint32_t (&w)[N / 4
 template <typename T, int Q, int A>
 __global__ void __launch_bounds__(kThreads)
     quantizeRowBlocks(const T* x, uint64_t xStride, T* y, uint64_t yStride, uint8_t* __restrict__ q, uint64_t qStride,
-                      uint8_t* __restrict__ scales, uint64_t blocks, uint32_t cols, uint32_t colBlocks, bool vectorX,
-                      bool vectorY, bool vectorQ) {
+                      uint8_t* __restrict__ scales, uint64_t blocks, uint32_t cols, uint32_t colBlocks, uint32_t alignX,
+                      uint32_t alignY, bool vectorQ) {
     const uint32_t lane = threadIdx.x % kGroup;
     const Place p = placeOf(blocks, colBlocks);
     const uint32_t left = p.active ? cols - p.col : 0u;
     Share<T> s;
-    s.load(x + p.row * xStride + p.col, left, lane, vectorX);
+    s.load(x + p.row * xStride + p.col, left, lane, alignX);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < Share<T>::kPieces; ++i)
@@ -144,7 +167,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int e = 0; e < kE; e += 2)
                 activation<A>(v[e], v[e + 1]);
-            Share<T>::store(y + p.row * yStride + p.col, i, v, left, lane, vectorY);
+            Share<T>::store(y + p.row * yStride + p.col, i, v, left, lane, alignY);
         }
     }
 }
@@ -154,7 +177,7 @@ __global__ void __launch_bounds__(kThreads)
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads)
     quantizeSquareBlocks(const T* __restrict__ x, uint64_t xStride, uint8_t* __restrict__ q, uint64_t qStride,
-                         uint8_t* __restrict__ scales, uint32_t rows, uint32_t cols, uint32_t colBlocks, bool vectorX,
+                         uint8_t* __restrict__ scales, uint32_t rows, uint32_t cols, uint32_t colBlocks, uint32_t alignX,
                          bool vectorQ) {
     constexpr int kE = kPer16<T>;
     constexpr uint32_t kLanes = kBlock / kE;               // lanes per row: 32 (fp32) or 16
@@ -165,18 +188,24 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t r0 = rowBlock * kBlock + threadIdx.x / kLanes;
     uint4 raw[kPasses];
     uint32_t top = 0;
+    if (alignX >= 16 && (rowBlock + 1) * uint64_t(kBlock) <= rows && (colBlock + 1) * uint64_t(kBlock) <= cols) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const uint64_t r = uint64_t(r0) + i * kRowsPerPass;
-        const T* src = x + r * xStride + c;
-        if (r < rows && vectorX && c + kE <= cols) {
-            raw[i] = __ldcs(reinterpret_cast<const uint4*>(src));
-        } else {
-            float v[kE];
+        for (int i = 0; i < kPasses; ++i)
+            raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + (uint64_t(r0) + i * kRowsPerPass) * xStride + c));
+    } else {
 #pragma unroll
-            for (int e = 0; e < kE; ++e)
-                v[e] = r < rows && c + e < cols ? toFloat(src[e]) : 0.0f;
-            raw[i] = pack16<T>(v); // exact: the values have type T
+        for (int i = 0; i < kPasses; ++i) {
+            const uint64_t r = uint64_t(r0) + i * kRowsPerPass;
+            const T* src = x + r * xStride + c;
+            if (r < rows && alignX >= 4 && c + kE <= cols) {
+                raw[i] = loadWords16(src, alignX);
+            } else {
+                float v[kE];
+#pragma unroll
+                for (int e = 0; e < kE; ++e)
+                    v[e] = r < rows && c + e < cols ? toFloat(src[e]) : 0.0f;
+                raw[i] = pack16<T>(v); // exact: the values have type T
+            }
         }
     }
 #pragma unroll
@@ -216,7 +245,7 @@ template <typename T, int A>
 __global__ void __launch_bounds__(kThreads)
     activationBackward(const T* dy, uint64_t dyStride, const uint8_t* __restrict__ q, uint64_t qStride,
                        const uint8_t* __restrict__ scales, T* dx, uint64_t dxStride, uint64_t blocks, uint32_t cols,
-                       uint32_t colBlocks, bool vectorDy, bool vectorDx, bool vectorQ) {
+                       uint32_t colBlocks, uint32_t alignDy, uint32_t alignDx, bool vectorQ) {
     constexpr int kE = Share<T>::kElems;
     const uint32_t lane = threadIdx.x % kGroup;
     const Place p = placeOf(blocks, colBlocks);
@@ -248,7 +277,7 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
     Share<T> s;
-    s.load(dy + p.row * dyStride + p.col, left, lane, vectorDy);
+    s.load(dy + p.row * dyStride + p.col, left, lane, alignDy);
 #pragma unroll
     for (int i = 0; i < Share<T>::kPieces; ++i) {
         float v[kE];
@@ -260,7 +289,7 @@ __global__ void __launch_bounds__(kThreads)
             activationSlope<A>(f, g);
             v[e] *= f, v[e + 1] *= g;
         }
-        Share<T>::store(dx + p.row * dxStride + p.col, i, v, left, lane, vectorDx);
+        Share<T>::store(dx + p.row * dxStride + p.col, i, v, left, lane, alignDx);
     }
 }
 
@@ -268,6 +297,11 @@ uint32_t rowGrid(uint64_t blocks) {
     const uint64_t grid = ceilDiv<uint64_t>(blocks, kGroups);
     require(grid <= 0x7FFFFFFFull, "too many blocks for one call");
     return uint32_t(grid);
+}
+
+// Bytes (16, 8, 4, or 0 for less) on which every row of a matrix starts.
+uint32_t alignmentOf(const void* p, uint64_t strideBytes) {
+    return rowsAlignedTo(p, strideBytes, 16) ? 16 : rowsAlignedTo(p, strideBytes, 8) ? 8 : rowsAlignedTo(p, strideBytes, 4) ? 4 : 0;
 }
 
 // Bytes that a lane stores or loads of q at once: 4 (fp32) or 8.
@@ -291,7 +325,7 @@ template <typename T, int Q, int A> void launchRows(const RowArgs& a, int type) 
     const uint64_t size = typeBytes(type);
     quantizeRowBlocks<T, Q, A><<<rowGrid(blocks), kThreads, 0, a.stream>>>(
         static_cast<const T*>(a.x), a.xStride, static_cast<T*>(a.y), a.yStride, a.q, a.qStride, a.scales, blocks, a.cols,
-        colBlocks, rowsAlignedTo(a.x, a.xStride * size, 16), rowsAlignedTo(a.y, a.yStride * size, 16),
+        colBlocks, alignmentOf(a.x, a.xStride * size), alignmentOf(a.y, a.yStride * size),
         rowsAlignedTo(a.q, a.qStride, pieceBytes(type)));
     checkCudaCall(cudaGetLastError());
 }
@@ -302,7 +336,7 @@ template <typename T, int Q> void launchSquares(const RowArgs& a, int type) {
     require(blocks <= 0x7FFFFFFFull, "too many blocks for one call");
     quantizeSquareBlocks<T, Q><<<uint32_t(blocks), kThreads, 0, a.stream>>>(
         static_cast<const T*>(a.x), a.xStride, a.q, a.qStride, a.scales, a.rows, a.cols, colBlocks,
-        rowsAlignedTo(a.x, a.xStride * typeBytes(type), 16), rowsAlignedTo(a.q, a.qStride, pieceBytes(type)));
+        alignmentOf(a.x, a.xStride * typeBytes(type)), rowsAlignedTo(a.q, a.qStride, pieceBytes(type)));
     checkCudaCall(cudaGetLastError());
 }
 
@@ -407,7 +441,7 @@ int tcc_activation_backward_int8(const void* grad_y, uint64_t grad_y_stride, int
                     activationBackward<T, decltype(f)::value><<<rowGrid(blocks), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
                         static_cast<const T*>(grad_y), grad_y_stride, reinterpret_cast<const uint8_t*>(q), q_stride,
                         scales, static_cast<T*>(grad_x), grad_x_stride, blocks, cols, colBlocks,
-                        rowsAlignedTo(grad_y, grad_y_stride * size, 16), rowsAlignedTo(grad_x, grad_x_stride * size, 16),
+                        alignmentOf(grad_y, grad_y_stride * size), alignmentOf(grad_x, grad_x_stride * size),
                         rowsAlignedTo(q, q_stride, pieceBytes(type)));
                     checkCudaCall(cudaGetLastError());
                 }

@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(32 * Few<MT>::kWarps)
     const uint64_t n0 = uint64_t(blockIdx.x) * L::kRows;
     const uint32_t kBlocks = (k + kBlock - 1) / kBlock;
     const uint32_t ring = dev::smemAddr(smem) + warp * L::kStages * L::kStageBytes;
-    // Copies of a block: a lane's 16-byte piece of rows lane / 8, + 4, ... Rows outside copy the last row
-    // instead: their sums go nowhere. Odd rows swap their 64-byte halves, for the banks.
+    // Copies of a block: a lane's 16-byte piece of rows lane / 8, + 4, ... Rows outside are not copied:
+    // their sums go nowhere. Odd rows swap their 64-byte halves, for the banks.
     const uint32_t piece = lane % 8, row0 = lane / 8;
     auto copy = [&](uint32_t kb, uint32_t stage) {
         const uint32_t to = ring + stage * L::kStageBytes + ((piece ^ ((row0 & 1) << 2)) * 16) + row0 * 128;
@@ -157,10 +157,12 @@ __global__ void __launch_bounds__(32 * Few<MT>::kWarps)
         const uint32_t bytes = c < k ? min(16u, k - c) : 0u, at = c < k ? c : 0u;
 #pragma unroll
         for (int i = 0; i < L::kRows / 4; ++i)
-            cpAsync16(to + 512 * i, b.data + min(n0 + row0 + 4 * i, uint64_t(n - 1)) * b.stride + at, bytes);
+            if (n0 + row0 + 4 * i < n)
+                cpAsync16(to + 512 * i, b.data + (n0 + row0 + 4 * i) * b.stride + at, bytes);
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i)
-            cpAsync16(to + L::kRows * 128 + 512 * i, a.data + uint64_t(min(row0 + 4 * i, m - 1)) * a.stride + at, bytes);
+            if (row0 + 4 * i < m)
+                cpAsync16(to + L::kRows * 128 + 512 * i, a.data + uint64_t(row0 + 4 * i) * a.stride + at, bytes);
     };
 #pragma unroll
     for (int i = 0; i < L::kStages; ++i) {
@@ -258,7 +260,10 @@ template <int MT> void launchFew(const Product& p) {
 // over the pair where CG = 2 (each CTA brings half of b's rows, which halves what an SM reads). Its
 // E8M0 scales are the blocks' own bytes: the hardware takes one scale per 32 elements of k, and a
 // block's four groups take the same one, so no scale is applied outside the tensor core and the sum
-// over all of k stays in one FP32 accumulator in tensor memory. Scales travel as words of four
+// over k stays in one FP32 accumulator in tensor memory. The tensor core cuts off what an addition
+// shifts out below the accumulator's last bit, about 1e-8 of the sum for every MMA (measured; 1.4e-6
+// after 128), so where the output shows it (fp32) the accumulator is emptied into registers, which
+// round to nearest, every kPass blocks. Scales travel as words of four
 // consecutive blocks per row, loaded by warps of their own, copied to tensor memory by the MMA thread
 // and picked by the byte selector of the instruction descriptor. Eight warps bring finished tiles into
 // registers, release the accumulator, and write them by TMA through 4 KB of shared memory each.
@@ -283,6 +288,7 @@ template <int BN_, int CG_> struct Tile {
     static constexpr int kNeed = kBarOff + 8 * kBars + 16 + 1024; // + alignment to 1024
     // At least half of the shared memory: a second CTA on the SM would wait for tensor memory.
     static constexpr int kBytes = kNeed > 120 * 1024 ? kNeed : 120 * 1024;
+    static constexpr uint32_t kPass = 12;                // blocks of k (48 MMAs); a multiple of 4, as scales come
     static constexpr int kScaleCols = 4 * kSlabs;
     static constexpr int kTmemCols = 512;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
@@ -415,7 +421,8 @@ __device__ __forceinline__ void storeTile(const ProductArgs& p, const CUtensorMa
     }
 }
 
-template <int BN, int CG, bool KN>
+// LONG: fp32 output of a k of more than kPass blocks, whose accumulators are summed in registers.
+template <int BN, int CG, bool KN, bool LONG>
 __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
     productTiles(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                  const __grid_constant__ CUtensorMap mapOut, const ProductArgs p) {
@@ -488,11 +495,18 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
         uint32_t stage = 0, phase = 0, slot = 0, slotPhase = 0, acc = 0, accPhase = 1;
         bool ok = true;
         for (uint32_t t = firstTile; t < tiles && ok; t += tileStep) {
-            if (!waitPhase(accEmpty + 8 * acc, accPhase))
-                break;
-            dev::tcFenceAfter();
-            const uint32_t d = tmem + acc * BN;
+            uint32_t passEnd = 0, d = 0; // the block of k before which the accumulator changes
             for (uint32_t kb = 0; kb < kBlocks; ++kb) {
+                const bool fresh = kb == passEnd;
+                if (fresh) {
+                    if (!waitPhase(accEmpty + 8 * acc, accPhase)) {
+                        ok = false;
+                        break;
+                    }
+                    dev::tcFenceAfter();
+                    d = tmem + acc * BN;
+                    passEnd = LONG ? min(kb + L::kPass, kBlocks) : kBlocks;
+                }
                 const uint32_t sa = scaleTmem + slot * L::kScaleCols, sb = sa + 4, byte = kb & 3;
                 if (byte == 0 && !waitPhase(scaleFull + 8 * slot, slotPhase)) {
                     ok = false;
@@ -516,11 +530,12 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         mmaScaled8<CG>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb,
-                                       j != 0 ? 1u : uint32_t(kb != 0));
+                                       j != 0 ? 1u : uint32_t(!fresh));
                 } else { // the last block ends inside
                     const uint32_t steps = (p.k - kb * kBlock + 31) / 32;
                     for (uint32_t j = 0; j < steps; ++j)
-                        mmaScaled8<CG>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb, (kb | j) != 0);
+                        mmaScaled8<CG>(elected, d, descA + 2 * j, descB + (KN ? 256 : 2) * j, idesc, sa, sb,
+                                       j != 0 || !fresh);
                 }
                 commitCluster<CG>(elected, empty + 8 * stage);
                 if (++stage == L::kStages)
@@ -530,11 +545,12 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                     if (++slot == L::kSlots)
                         slot = 0, slotPhase ^= 1;
                 }
+                if (kb + 1 == passEnd) {
+                    commitCluster<CG>(elected, accFull + 8 * acc);
+                    if (++acc == L::kAcc)
+                        acc = 0, accPhase ^= 1;
+                }
             }
-            if (ok)
-                commitCluster<CG>(elected, accFull + 8 * acc);
-            if (++acc == L::kAcc)
-                acc = 0, accPhase ^= 1;
         }
     } else if (warp == L::kMmaWarp) {
         // The second CTA of a pair tells the first that its stages and scales are there.
@@ -615,30 +631,49 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                 __syncwarp();
                 biasAt = n0;
             }
-            if (!waitPhase(accFull + 8 * acc, phase))
-                break;
-            dev::tcFenceAfter();
-            const uint32_t from = tmem + acc * BN + half * L::kHalf + (quarter << 21); // lanes in bits 16-31
             uint32_t r[L::kHalf];
-            if constexpr (L::kHalf == 16) {
-                dev::tcLoad32x32bx16(from, r);
-            } else {
+            bool ok = true;
+            for (uint32_t kb = 0; kb < (LONG ? kBlocks : 1u); kb += L::kPass) {
+                if (!waitPhase(accFull + 8 * acc, phase)) {
+                    ok = false;
+                    break;
+                }
+                dev::tcFenceAfter();
+                const uint32_t from = tmem + acc * BN + half * L::kHalf + (quarter << 21); // lanes in bits 16-31
+                if (!LONG || kb == 0) {
+                    if constexpr (L::kHalf == 16) {
+                        dev::tcLoad32x32bx16(from, r);
+                    } else {
 #pragma unroll
-                for (int i = 0; i < L::kHalf / 32; ++i)
-                    tcLoad32x32bx32(from + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * i));
+                        for (int i = 0; i < L::kHalf / 32; ++i)
+                            tcLoad32x32bx32(from + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * i));
+                    }
+                    dev::tcWaitLd();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < L::kHalf; i += 8) {
+                        uint32_t more[8];
+                        tcLoad32x32bx8(from + i, more);
+                        dev::tcWaitLd();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            r[i + j] = __float_as_uint(__uint_as_float(r[i + j]) + __uint_as_float(more[j]));
+                    }
+                }
+                dev::tcFenceBefore();
+                __syncwarp();
+                if (lane == 0)
+                    arriveLeader<CG>(accEmpty + 8 * acc);
+                if (++acc == L::kAcc)
+                    acc = 0, phase ^= 1;
             }
-            dev::tcWaitLd();
-            dev::tcFenceBefore();
-            __syncwarp();
-            if (lane == 0)
-                arriveLeader<CG>(accEmpty + 8 * acc);
-            if (++acc == L::kAcc)
-                acc = 0, phase ^= 1;
+            if (!ok)
+                break;
             const uint64_t row0 = m0 + 128 * rank + 32 * quarter;
             if (row0 < p.m && n0 < p.n) {
-                if (p.outType == TCC_BF16)
+                if (!LONG && p.outType == TCC_BF16)
                     storeTile<L, __nv_bfloat16>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
-                else if (p.outType == TCC_F32)
+                else if (LONG || p.outType == TCC_F32)
                     storeTile<L, float>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
                 else
                     storeTile<L, __half>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
@@ -690,7 +725,6 @@ template <int BN, int CG, bool KN> void launchTiles(const Product& p) {
                              outBytes, p.m, p.n, p.outStride, 32, width / outBytes,
                              width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
     }
-    allowSharedMemory<productTiles<BN, CG, KN>>(L::kBytes);
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(CG * std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors() / CG));
     config.blockDim = dim3(L::kThreads);
@@ -701,7 +735,13 @@ template <int BN, int CG, bool KN> void launchTiles(const Product& p) {
     attr.val.clusterDim.x = CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN>, mapA, mapB, mapOut, args));
+    if (p.outType == TCC_F32 && kBlocks > L::kPass) {
+        allowSharedMemory<productTiles<BN, CG, KN, true>>(L::kBytes);
+        checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN, true>, mapA, mapB, mapOut, args));
+    } else {
+        allowSharedMemory<productTiles<BN, CG, KN, false>>(L::kBytes);
+        checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN, false>, mapA, mapB, mapOut, args));
+    }
 }
 
 void launchProduct(const Product& p) {

@@ -26,10 +26,12 @@ SHAPES = [(1, 1), (1, 128), (3, 127), (130, 129), (257, 384), (64, 1000), (5, 41
 @pytest.mark.parametrize("rows,cols", SHAPES)
 def test_quantize_blocks(rows, cols, dtype, kind, block_rows):
     x = D.make(rows, cols, D.TYPES[dtype], rows + cols)
-    for stride, offset in ((D.up16(cols), 0), (cols + 3, 1)):
+    for stride, offset, x_stride, x_offset in ((D.up16(cols), 0, D.up16(cols), 0), (cols + 3, 1, cols + 5, 1),
+                                               (D.up16(cols) + 8, 8, D.up16(cols) + 4, 4),
+                                               (D.up16(cols) + 4, 4, D.up16(cols) + 2, 2)):
         q = D.strided(rows, cols, D.FP8[kind], stride, offset)
         scales = torch.zeros(-(-rows // block_rows), -(-cols // 128), dtype=torch.uint8, device="cuda")
-        xs = D.strided(rows, cols, x.dtype, cols + (8 if offset == 0 else 5), 0 if offset == 0 else 1)
+        xs = D.strided(rows, cols, x.dtype, x_stride, x_offset)
         xs.copy_(x)
         T.quantize_blocks_fp8(xs, q, scales, block_rows=block_rows)
         want, bytes_ = D.quantize(x, kind, block_rows)
@@ -211,9 +213,9 @@ def function_bound(x, kind):
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 129), (33, 128), (130, 257), (50, 1001)])
 def test_checkpoint_and_backward(rows, cols, dtype, kind):
     dt = D.TYPES[dtype]
-    for aligned in (True, False):
+    for stride, offset in ((D.up16(cols), 0), (cols + 1, 1), (D.up16(cols) + 4, 4), (D.up16(cols) + 2, 2)):
         def held(t):
-            return D.strided(rows, cols, t, D.up16(cols) if aligned else cols + 1, 0 if aligned else 1)
+            return D.strided(rows, cols, t, stride, offset)
 
         x, y, q, dy, dx = held(dt), held(dt), held(torch.int8), held(dt), held(dt)
         x.copy_(D.make(rows, cols, dt, rows * cols))
