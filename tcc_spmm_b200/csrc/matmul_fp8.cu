@@ -288,7 +288,7 @@ template <int BN_, int CG_> struct Tile {
     static constexpr int kNeed = kBarOff + 8 * kBars + 16 + 1024; // + alignment to 1024
     // At least half of the shared memory: a second CTA on the SM would wait for tensor memory.
     static constexpr int kBytes = kNeed > 120 * 1024 ? kNeed : 120 * 1024;
-    static constexpr uint32_t kPass = 12;                // blocks of k (48 MMAs); a multiple of 4, as scales come
+    static constexpr uint32_t kPass = 16;                // blocks of k (64 MMAs); a multiple of 4, as scales come
     static constexpr int kScaleCols = 4 * kSlabs;
     static constexpr int kTmemCols = 512;
     static constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
