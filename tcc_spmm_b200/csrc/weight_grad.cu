@@ -121,40 +121,53 @@ template <typename T> __device__ __forceinline__ Quad<T> loadQuad(uint32_t addr)
     return v;
 }
 
-__device__ __forceinline__ uint32_t packBf16(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
+// The upper halves of two floats (their bf16 parts, cut off) as a pair, and what is left of them: a
+// float's 24 bits are three such parts of 8, and every difference is exact.
+__device__ __forceinline__ uint32_t upperPair(float lo, float hi) {
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
-// What is left of a pair after its bf16 rounding (exact).
-__device__ __forceinline__ void subtractBf16(float& lo, float& hi, uint32_t packed) {
-    lo -= __uint_as_float(packed << 16);
-    hi -= __uint_as_float(packed & 0xFFFF0000u);
+__device__ __forceinline__ float withoutUpper(float v) {
+    return v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
 }
 
-// Column c (0..3) of two rows' quads as P bf16 pairs (row u in the low half). A part that is not
-// finite because the value is not leaves the later parts zero.
-template <typename T> __device__ __forceinline__ void splitPair(const Quad<T>& u, const Quad<T>& v, int c, uint32_t (&part)[kParts<T>]) {
-    if constexpr (sizeof(T) == 4) {
-        float a = __uint_as_float(u.w[c]), b = __uint_as_float(v.w[c]);
-        part[0] = packBf16(a, b);
-        subtractBf16(a, b, part[0]);
-        a = fabsf(a) < INFINITY ? a : 0.0f, b = fabsf(b) < INFINITY ? b : 0.0f;
-        part[1] = packBf16(a, b);
-        subtractBf16(a, b, part[1]);
-        part[2] = packBf16(a, b);
+// Column c (0..3) of two rows' quads as P bf16 pairs (row u in the low half). CHECK: a value that is
+// not finite leaves its later parts zero (infinity minus infinity would make them NaN).
+template <typename T, bool CHECK>
+__device__ __forceinline__ void splitPair(const Quad<T>& u, const Quad<T>& v, int c, uint32_t (&part)[kParts<T>]) {
+    if constexpr (kParts<T> == 1) {
+        part[0] = __byte_perm(u.w[c / 2], v.w[c / 2], c % 2 ? 0x7632 : 0x5410);
     } else {
-        const uint32_t pair = __byte_perm(u.w[c / 2], v.w[c / 2], c % 2 ? 0x7632 : 0x5410);
-        if constexpr (kParts<T> == 1) {
-            part[0] = pair;
+        float a, b;
+        if constexpr (sizeof(T) == 4) {
+            a = __uint_as_float(u.w[c]), b = __uint_as_float(v.w[c]);
         } else {
+            const uint32_t pair = __byte_perm(u.w[c / 2], v.w[c / 2], c % 2 ? 0x7632 : 0x5410);
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
-            float a = f.x, b = f.y;
-            part[0] = packBf16(a, b);
-            subtractBf16(a, b, part[0]);
-            a = fabsf(a) < INFINITY ? a : 0.0f, b = fabsf(b) < INFINITY ? b : 0.0f;
-            part[1] = packBf16(a, b);
+            a = f.x, b = f.y;
         }
+        part[0] = upperPair(a, b);
+        if constexpr (CHECK) { // a NaN whose upper half says infinity still has to stay one
+            part[0] |= (a != a ? 0x7FFFu : 0u) | (b != b ? 0x7FFF0000u : 0u);
+            a = fabsf(a) < INFINITY ? a : 0.0f, b = fabsf(b) < INFINITY ? b : 0.0f;
+        }
+        a = withoutUpper(a), b = withoutUpper(b);
+        part[1] = upperPair(a, b);
+        if constexpr (kParts<T> == 3)
+            part[2] = upperPair(withoutUpper(a), withoutUpper(b));
     }
+}
+// Whether any of a warp's quads may hold a value that is not finite: exponents are looked at together,
+// so large finite ones can raise it too, which only costs the checks.
+template <typename T> __device__ __forceinline__ bool mayNotBeFinite(const Quad<T> (&q)[4]) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < int(sizeof(T)); ++j)
+            any |= q[i].w[j];
+    const bool raised = sizeof(T) == 4 ? (any & 0x7F800000u) == 0x7F800000u
+                                       : (any & 0x7C00u) == 0x7C00u || (any & 0x7C000000u) == 0x7C000000u;
+    return __any_sync(0xFFFFFFFFu, raised);
 }
 
 // Four INT8 elements times a power of two (a bf16 pair) in bf16: low 7 bits under the exponent
@@ -315,17 +328,24 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < kJ; ++j) {
                 const Quad<T>(&q)[4] = quads[j];
+                auto put = [&](auto check) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t out[4][L::kP];
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t out[4][L::kP];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) // lane t / 4 + 8 (x / 2), column 8 j + 2 q4 + x % 2
-                        splitPair<T>(q[2 * (x % 2)], q[2 * (x % 2) + 1], 2 * half + x / 2, out[x]);
+                        for (int x = 0; x < 4; ++x) // lane t / 4 + 8 (x / 2), column 8 j + 2 q4 + x % 2
+                            splitPair<T, decltype(check)::value != 0>(q[2 * (x % 2)], q[2 * (x % 2) + 1], 2 * half + x / 2,
+                                                                      out[x]);
 #pragma unroll
-                    for (int m = 0; m < L::kP; ++m)
-                        tcStore16x256b(to + m * (L::kRows / 2) + 8 * (j0 + j) + (half << 20), out[0][m], out[1][m], out[2][m],
-                                       out[3][m]);
-                }
+                        for (int m = 0; m < L::kP; ++m)
+                            tcStore16x256b(to + m * (L::kRows / 2) + 8 * (j0 + j) + (half << 20), out[0][m], out[1][m],
+                                           out[2][m], out[3][m]);
+                    }
+                };
+                if (L::kP > 1 && mayNotBeFinite<T>(q))
+                    put(Const<1>{});
+                else
+                    put(Const<0>{});
             }
             }
             dev::tcWaitSt();

@@ -330,6 +330,30 @@ def test_weight_grad_nan_block():
     assert (dw[:, :128] == 300).all() and dw[:, 128:].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_weight_grad_not_finite_gradient(dtype):
+    """Infinities and NaN of dy arrive as such: inf times a positive element is inf, times zero NaN. So does the
+    largest finite value."""
+    rows, n, k = 300, 40, 130
+    dt = D.TYPES[dtype]
+    q = torch.ones(rows, k, dtype=torch.int8, device="cuda")
+    q[:, 1] = -3
+    q[:, 2] = 0
+    scales = torch.full((rows, 2), 127, dtype=torch.uint8, device="cuda")
+    dy = torch.zeros(rows, n, device="cuda", dtype=dt)
+    dy[5, 0], dy[6, 1], dy[7, 2], dy[200, 3] = float("inf"), -float("inf"), float("nan"), torch.finfo(dt).max
+    dy[8, 4] = 1.0
+    dw = torch.empty(n, k, device="cuda")
+    T.weight_grad_int8(dy, q, scales, dw)
+    want = dy.float().t() @ q.float()
+    want[3] = torch.finfo(dt).max * q[0].float()
+    assert torch.equal(torch.nan_to_num(dw, nan=1.5), torch.nan_to_num(want, nan=1.5))
+    if dtype == "fp32":  # a NaN whose upper half alone would be an infinity
+        dy[7, 2] = torch.tensor([0x7F800001], dtype=torch.int32, device="cuda").view(torch.float32)[0]
+        T.weight_grad_int8(dy, q, scales, dw)
+        assert dw[2].isnan().all()
+
+
 # ---- sizes of zero, refusals ------------------------------------------------------------------------
 def test_empty():
     e4 = torch.float8_e4m3fn
