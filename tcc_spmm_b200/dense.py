@@ -29,17 +29,17 @@ LAYOUTS = {"nk": 0, "kn": 1}
 
 # torch, its raw-stream and current-device queries, and the type codes, once an operator is used
 _torch = _raw_stream = _current_device = _call = None
-_TYPES: dict = {}
+_FLOATS: dict = {}
+_FP8: dict = {}
 _SCALES: set = set()
-_FLOATS, _FP8 = (0, 1, 2), (3, 4)
 
 
 def _load():
     global _torch, _raw_stream, _current_device, _call
     import torch
 
-    _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3,
-                   torch.float8_e5m2: 4})
+    _FLOATS.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    _FP8.update({torch.float8_e4m3fn: 3, torch.float8_e5m2: 4})
     _SCALES.update((torch.uint8, torch.float8_e8m0fnu))
     _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
     _call = N.lib().tcc_dense8_call
@@ -75,7 +75,13 @@ def _matrix(name: str, t, device: int = -1) -> tuple:
 
 def _shaped(name: str, t, rows: int, cols: int, device: int) -> int:
     """The row stride of a 2-D CUDA operand that must have this shape."""
-    r, c, stride, _ = _matrix(name, t, device)
+    try:
+        row_stride, col_stride = t.stride()
+        if col_stride == 1 and row_stride >= cols and rows > 1 and t.shape == (rows, cols) and t.get_device() == device:
+            return row_stride
+    except (AttributeError, TypeError, ValueError, RuntimeError):
+        pass
+    r, c, stride, _ = _matrix(name, t, device)  # the special cases, and the messages
     if r != rows or c != cols:
         _refuse(f"{name} has shape {(r, c)}, expected {(rows, cols)}")
     return stride
@@ -83,24 +89,24 @@ def _shaped(name: str, t, rows: int, cols: int, device: int) -> int:
 
 def _scales(name: str, t, device: int, rows: int, cols: int, row_blocks: bool = True, square_blocks: bool = True) -> int:
     """Checks the scale bytes of a [rows, cols] matrix and returns the rows per block."""
-    if t.dtype not in _SCALES:
-        _refuse(f"{name} must hold scale bytes (uint8 or float8_e8m0fnu)")
-    if t.get_device() != device:
-        _refuse(f"{name} is on {t.device}, expected cuda:{device}")
     wide = (cols + 127) >> 7
-    shape = tuple(t.shape)
-    if t.is_contiguous():
+    if t.dtype in _SCALES and t.get_device() == device and t.is_contiguous():
+        shape = t.shape
         if row_blocks and shape == (rows, wide):
             return 1
         if square_blocks and shape == ((rows + 127) >> 7, wide):
             return BLOCK
+    if t.dtype not in _SCALES:
+        _refuse(f"{name} must hold scale bytes (uint8 or float8_e8m0fnu)")
+    if t.get_device() != device:
+        _refuse(f"{name} is on {t.device}, expected cuda:{device}")
     want = [(rows, wide)] * row_blocks + [((rows + 127) >> 7, wide)] * square_blocks
-    _refuse(f"{name} has shape {shape}, expected contiguous {' or '.join(map(str, want))}")
+    _refuse(f"{name} has shape {tuple(t.shape)}, expected contiguous {' or '.join(map(str, want))}")
 
 
-def _type(name: str, t, allowed) -> int:
-    code = _TYPES.get(t.dtype)
-    if code not in allowed:
+def _type(name: str, t, types: dict) -> int:
+    code = types.get(t.dtype)
+    if code is None:
         _refuse(f"{name} has unsupported type {t.dtype}")
     return code
 
@@ -170,16 +176,11 @@ def matmul_fp8_blocks(a, a_scales, b, b_scales, output, bias=None, b_layout: str
             output.data_ptr(), ot, os_, m, n, k)
 
 
-def _int8(name: str, q) -> None:
-    if q.dtype != _torch.int8:
-        _refuse(f"{name} must be int8")
-
-
 def _pair(name: str, t, other, stride: int, other_stride: int) -> None:
     """An output of the input's type that is the input itself or no view of it from the same start."""
     if t.dtype != other.dtype:
         _refuse(f"{name} must have its input's type")
-    if t.data_ptr() == other.data_ptr() and stride != other_stride:
+    if stride != other_stride and t.data_ptr() == other.data_ptr():
         _refuse(f"{name} may be its input itself, not another view of it")
 
 
@@ -204,7 +205,8 @@ def activation_checkpoint_int8(x, y, q, scales, activation: str = "gelu", stream
         ys, y_ptr = _shaped("y", y, rows, cols, device), y.data_ptr()
         _pair("y", y, x, ys, xs)
     qs = _shaped("q", q, rows, cols, device)
-    _int8("q", q)
+    if q.dtype != _torch.int8:
+        _refuse("q must be int8")
     _scales("scales", scales, device, rows, cols, True, False)
     _launch(device, stream, _CHECKPOINT, x.data_ptr(), xs, y_ptr, ys, xt, q.data_ptr(), qs,
             scales.data_ptr(), rows, cols, code)
@@ -226,7 +228,8 @@ def activation_backward_int8(grad_y, q, scales, grad_x, activation: str = "gelu"
     xs = _shaped("grad_x", grad_x, rows, cols, device)
     _pair("grad_x", grad_x, grad_y, xs, gs)
     qs = _shaped("q", q, rows, cols, device)
-    _int8("q", q)
+    if q.dtype != _torch.int8:
+        _refuse("q must be int8")
     _scales("scales", scales, device, rows, cols, True, False)
     _launch(device, stream, _BACKWARD, grad_y.data_ptr(), gs, gt, q.data_ptr(), qs,
             scales.data_ptr(), grad_x.data_ptr(), xs, rows, cols, code)
@@ -255,7 +258,8 @@ def weight_grad_int8(grad_y, q, scales, grad_w, accumulate: bool = False, worksp
     q_rows, k, qs, _ = _matrix("q", q, device)
     if q_rows != rows:
         _refuse(f"q has {q_rows} rows, grad_y {rows}")
-    _int8("q", q)
+    if q.dtype != _torch.int8:
+        _refuse("q must be int8")
     ws = _shaped("grad_w", grad_w, n, k, device)
     if grad_w.dtype != _torch.float32:
         _refuse("grad_w must be fp32")
