@@ -97,7 +97,9 @@ template <typename T> struct Share {
     static __device__ __forceinline__ void store(T* row, int i, const float (&v)[kElems], uint32_t left, uint32_t lane,
                                                  uint32_t align) {
         const uint32_t c = column(i, lane);
-        if (align >= 4 && c + kElems <= left) {
+        if (align >= 16 && left >= kBlock) {
+            __stcs(reinterpret_cast<uint4*>(row + c), pack16<T>(v));
+        } else if (align >= 4 && c + kElems <= left) {
             storeWords16(row + c, pack16<T>(v), align);
         } else {
 #pragma unroll
