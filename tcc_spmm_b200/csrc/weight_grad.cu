@@ -625,7 +625,8 @@ Plan planOf(uint32_t rows, uint32_t n, uint32_t k) {
     const uint32_t steps = std::max(1u, ceilDiv(rows, 64u));
     const double stepUs = 0.4, tileUs = p.cg * 128.0 * 256 * 4 * 2 / 5e6; // 64 rows; a partial tile out and in
     double best = 0;
-    for (uint32_t splits = 1; splits <= steps && splits <= 296; ++splits) {
+    const uint32_t most = uint32_t(std::min(double(steps), std::max(4.0, 2 * kSms / (tiles * p.cg))));
+    for (uint32_t splits = 1; splits <= most; ++splits) {
         const uint32_t per = ceilDiv(steps, splits);
         if (ceilDiv(steps, per) != splits)
             continue;
