@@ -318,7 +318,7 @@ struct ProductArgs {
     void* out;
     uint64_t outStride;
     int outType;
-    bool outTma; // output rows start on 16 bytes: written by TMA
+    bool outTma; // output rows start and end on 16 bytes: written by TMA
     uint32_t m, n, k, tilesM, tilesN;
     uint32_t idesc;
 };
@@ -705,7 +705,8 @@ template <int BN, int CG, bool KN> void launchTiles(const Product& p) {
     args.out = p.out;
     args.outStride = p.outStride;
     args.outType = p.outType;
-    args.outTma = rowsAlignedTo(p.out, p.outStride * outBytes, 16) && p.outStride < (1ull << 38);
+    // A TMA store writes whole 16-byte pieces of a row: n has to end one, or the next columns change.
+    args.outTma = rowsAlignedTo(p.out, p.outStride * outBytes, 16) && p.n * uint64_t(outBytes) % 16 == 0 && p.outStride < (1ull << 38);
     args.m = p.m, args.n = p.n, args.k = p.k;
     args.tilesM = ceilDiv<uint32_t>(p.m, 128 * CG);
     args.tilesN = ceilDiv<uint32_t>(p.n, BN);

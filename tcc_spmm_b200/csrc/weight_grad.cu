@@ -43,7 +43,8 @@ struct GradArgs {
     uint32_t rows, n, k;
     uint32_t tilesN, tilesK, rowsPerSplit;
     bool accumulate;
-    bool dwVector; // rows of dw start on 16 bytes
+    int dyAlign, qAlign; // bytes (up to 8 and 4) that every row of dy and of q starts on, read where TMA is not used
+    bool dwTma; // rows of dw start and end on 16 bytes: written by TMA
 };
 
 template <uint32_t V> struct Const { static constexpr uint32_t value = V; };
@@ -83,7 +84,7 @@ template <typename T, int CG> struct GradTile {
     // 128 sums.
     static constexpr int kRegs = 72, kRegsEpilogue = 152, kRegsA = 40, kRegsB = 40, kRegsIssue = 40;
     static_assert(2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * kRegs, "the shares exceed the launch's registers");
-    static_assert(kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
+    static_assert(kRaw * kRawBytes >= 8 * 4096 && kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
 };
 
 // kind::f16 with FP32 accumulators (bits 4-5 = 1), bf16 A and B (bits 7-9 and 10-12 = 1), B
@@ -209,9 +210,88 @@ __device__ __forceinline__ uint32_t operandRow(uint32_t r) { // its inverse: raw
     return (r & ~15u) | ((r & 6u) << 1) | ((r & 8u) >> 2) | (r & 1u);
 }
 
+// One row's pieces of W bytes (8, 4, 2 or 1), 32 W apart, to shared memory at place(byte of the row);
+// `have` bytes exist from the lane's first piece on, and zeros go behind them. 8 and 4 bytes go by
+// asynchronous copies, whose address has to be valid even where nothing is read; 2 and 1 through
+// registers, all loads before the stores.
+template <int W, int PIECES, typename Place>
+__device__ __forceinline__ void copyRow(const uint8_t* src, const void* valid, int have, uint32_t lane, Place place) {
+    if constexpr (W >= 4) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const uint32_t bytes = uint32_t(max(0, min(W, have - 32 * i * W)));
+            const void* from = bytes != 0 ? static_cast<const void*>(src + 32 * i * W) : valid;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(place((32 * i + lane) * W)), "l"(from), "n"(W),
+                         "r"(bytes)
+                         : "memory");
+        }
+    } else {
+        uint32_t v[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const uint8_t* at = src + 32 * i * W;
+            v[i] = have - 32 * i * W < W ? 0u : W == 2 ? uint32_t(__ldg(reinterpret_cast<const unsigned short*>(at))) : uint32_t(__ldg(at));
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const uint32_t to = place((32 * i + lane) * W);
+            if constexpr (W == 2)
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<unsigned short>(v[i])) : "memory");
+            else
+                stsU8(to, v[i]);
+        }
+    }
+}
+// One of the three warps that fill raw stages without TMA: rows warp, warp + 3, ..., pieces of WA bytes
+// of dy and WB bytes of q. Every lane arrives on the stage's barrier once its copies have landed.
+template <typename T, int CG, int WA, int WB>
+__device__ __forceinline__ void loadRaw(const GradArgs& p, uint32_t base, uint32_t rawFull, uint32_t rawEmpty, uint32_t warp,
+                                        uint32_t lane, uint64_t begin, uint64_t end, uint32_t stages, uint32_t n0,
+                                        uint32_t kMine) {
+    using L = GradTile<T, CG>;
+    constexpr int kPiecesA = 128 * int(sizeof(T)) / (32 * WA), kPiecesB = L::kBCols / (32 * WB);
+    const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, col = kMine / kBlock;
+    const uint32_t scaleRow = warp + 3 * lane; // the lane's row for the scales
+    const int bytesA = n0 < p.n ? int(min(p.n - n0, 128u) * sizeof(T)) - int(lane) * WA : 0;
+    const int bytesB = kMine < p.k ? int(min(p.k - kMine, uint32_t(L::kBCols))) - int(lane) * WB : 0;
+    const uint8_t* dy = static_cast<const uint8_t*>(p.dy) + uint64_t(n0) * sizeof(T) + lane * WA;
+    const uint8_t* q = p.q + kMine + lane * WB;
+    uint32_t raw = 0, phase = 1;
+    for (uint32_t it = 0; it < stages; ++it) {
+        if (!waitPhase(rawEmpty + 8 * raw, phase))
+            break;
+        const uint32_t to = base + L::kRawOff + raw * L::kRawBytes, scales = base + L::kScaleOff + raw * L::kScaleBytes;
+        const uint64_t row0 = begin + uint64_t(it) * L::kRows;
+        uint32_t scale[L::kBBoxes];
+#pragma unroll
+        for (int box = 0; box < L::kBBoxes; ++box)
+            scale[box] = scaleRow < uint32_t(L::kRows) && row0 + scaleRow < end && col + box < kBlocks
+                             ? uint32_t(__ldg(p.scales + (row0 + scaleRow) * kBlocks + col + box)) : 127u;
+        for (uint32_t r = warp; r < uint32_t(L::kRows); r += 3) {
+            const uint64_t row = row0 + r;
+            const bool in = row < end;
+            copyRow<WA, kPiecesA>(dy + row * p.dyStride * sizeof(T), p.dy, in ? bytesA : 0, lane, [&](uint32_t byte) {
+                return to + byte / 128 * L::kBox + r * 128 + ((byte % 128) ^ ((r & 7) << 4));
+            });
+            copyRow<WB, kPiecesB>(q + row * p.qStride, p.q, in ? bytesB : 0, lane, [&](uint32_t byte) {
+                return to + (L::kABoxes + byte / 128) * L::kBox + r * 128 + byte % 128;
+            });
+        }
+#pragma unroll
+        for (int box = 0; box < L::kBBoxes; ++box)
+            if (scaleRow < uint32_t(L::kRows))
+                stsU32(scales + 4 * (box * L::kRows + scaleRow), scalePair(scale[box]));
+        dev::cpAsyncArriveNoinc(rawFull + 8 * raw);
+        if (++raw == L::kRaw)
+            raw = 0, phase ^= 1;
+    }
+    dev::cpAsyncWaitAll(); // none may be on its way when the CTA exits
+}
+
 template <typename T, int CG, bool TMA>
 __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
-    gradTiles(const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ CUtensorMap mapQ, const GradArgs p) {
+    gradTiles(const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ CUtensorMap mapQ,
+              const __grid_constant__ CUtensorMap mapDw, const GradArgs p) {
     using L = GradTile<T, CG>;
     extern __shared__ unsigned char smemRaw[];
     const uint32_t base = (dev::smemAddr(smemRaw) + 1023u) & ~1023u;
@@ -223,7 +303,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kRaw; ++i)
-            dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 3), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
+            dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 96), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
         for (int i = 0; i < L::kStages; ++i)
             dev::mbarInit(full + 8 * i, 8), dev::mbarInit(empty + 8 * i, 1), dev::mbarInit(peerFull + 8 * i, 1);
         dev::mbarInit(accFull, 1), dev::mbarInit(accEmpty, 8 * CG);
@@ -278,23 +358,47 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 out[128 * i] = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+        } else if (ok && p.dwTma) {
+            // Boxes of 32 x 32 through the raw ring, which nothing uses any more, swizzled as the map says;
+            // accumulate adds them where they go.
+            const uint32_t buf = base + L::kRawOff + warp * 4096, r = laneColumn(lane);
+#pragma unroll
+            for (int box = 0; box < 4; ++box) {
+                const uint32_t x = k0 + 128 * half + 32 * box, y = n0 + 32 * quarter;
+                if (lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(buf + r * 128 + ((j ^ r) & 7) * 16), "f"(sum[32 * box + 4 * j]),
+                                 "f"(sum[32 * box + 4 * j + 1]), "f"(sum[32 * box + 4 * j + 2]),
+                                 "f"(sum[32 * box + 4 * j + 3])
+                                 : "memory");
+                dev::fenceProxyAsyncShared();
+                __syncwarp();
+                if (lane == 0 && x < p.k && y < p.n) {
+                    if (p.accumulate)
+                        asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
+                                     ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
+                                     : "memory");
+                    else
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                                     ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
+                                     : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            }
+            if (lane == 0) // shared memory stays until the copies have read it
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
         } else if (ok && row < p.n) {
 #pragma unroll
-            for (int i = 0; i < 128; i += 4) {
+            for (int i = 0; i < 128; ++i) {
                 const uint32_t col = k0 + 128 * half + i;
-                float* out = p.dw + row * p.dwStride + col;
-                if (p.dwVector && col + 4 <= p.k) {
-                    float4 v = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
-                    if (p.accumulate) {
-                        const float4 was = *reinterpret_cast<const float4*>(out);
-                        v = make_float4(v.x + was.x, v.y + was.y, v.z + was.z, v.w + was.w);
-                    }
-                    *reinterpret_cast<float4*>(out) = v;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < p.k)
-                            out[j] = sum[i + j] + (p.accumulate ? out[j] : 0.0f);
+                if (col < p.k) {
+                    float* out = p.dw + row * p.dwStride + col;
+                    *out = sum[i] + (p.accumulate ? *out : 0.0f);
                 }
             }
         }
@@ -520,44 +624,17 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                     }
             }
         } else {
-            // ---- raw stages element by element, for rows that do not start on 16 bytes: three warps ----
-            uint32_t raw = 0, phase = 1;
-            for (uint32_t it = 0; it < stages; ++it) {
-                if (!waitPhase(rawEmpty + 8 * raw, phase))
-                    break;
-                const uint32_t to = base + L::kRawOff + raw * L::kRawBytes;
-                for (uint32_t r = warp - L::kLoadWarp; r < uint32_t(L::kRows); r += 3) {
-                    const uint64_t row = begin + uint64_t(it) * L::kRows + r;
-                    const bool in = row < end;
-                    const T* dy = static_cast<const T*>(p.dy) + row * p.dyStride + n0;
-                    for (uint32_t c = lane; c < 128; c += 32) {
-                        const uint32_t byte = c * sizeof(T), at = to + byte / 128 * L::kBox + r * 128 + ((byte % 128) ^ ((r & 7) << 4));
-                        const bool valid = in && n0 + c < p.n;
-                        if constexpr (sizeof(T) == 4) {
-                            const uint32_t v = valid ? __ldg(reinterpret_cast<const uint32_t*>(dy) + c) : 0u;
-                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-                        } else {
-                            const unsigned short v = valid ? __ldg(reinterpret_cast<const unsigned short*>(dy) + c) : 0;
-                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
-                        }
-                    }
-                    if (lane < uint32_t(L::kBBoxes)) {
-                        const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock, col = kMine / kBlock + lane;
-                        stsU32(base + L::kScaleOff + raw * L::kScaleBytes + 4 * (lane * L::kRows + r),
-                               scalePair(in && col < kBlocks ? uint32_t(__ldg(p.scales + row * kBlocks + col)) : 127u));
-                    }
-                    const uint8_t* q = p.q + row * p.qStride + kMine;
-                    for (uint32_t c = lane; c < uint32_t(L::kBCols); c += 32) {
-                        const uint32_t at = to + (L::kABoxes + c / 128) * L::kBox + r * 128 + c % 128;
-                        stsU8(at, in && kMine + c < p.k ? uint32_t(__ldg(q + c)) : 0u);
-                    }
-                }
-                __syncwarp();
-                if (lane == 0)
-                    dev::mbarArrive(rawFull + 8 * raw);
-                if (++raw == L::kRaw)
-                    raw = 0, phase ^= 1;
-            }
+            // ---- raw stages by three warps, for rows that do not start on 16 bytes: pieces of dy and of q
+            // as wide as their rows' alignment allows ----
+            if (p.dyAlign >= 8)
+                p.qAlign >= 4 ? loadRaw<T, CG, 8, 4>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine)
+                              : loadRaw<T, CG, 8, 1>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine);
+            else if (p.dyAlign >= 4)
+                p.qAlign >= 4 ? loadRaw<T, CG, 4, 4>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine)
+                              : loadRaw<T, CG, 4, 1>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine);
+            else if constexpr (sizeof(T) == 2)
+                p.qAlign >= 4 ? loadRaw<T, CG, 2, 4>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine)
+                              : loadRaw<T, CG, 2, 1>(p, base, rawFull, rawEmpty, warp - L::kLoadWarp, lane, begin, end, stages, n0, kMine);
         }
     }
     __syncwarp();
@@ -659,7 +736,9 @@ void launchTiles(const GradArgs& g, const Plan& p, int type, cudaStream_t stream
         throw CudaError("weight_grad_int8 was built with an unexpected register count");
     const uint64_t grid = uint64_t(p.tilesN) * p.tilesK * p.splits * CG;
     require(grid <= 0x7FFFFFFFull, "too many output tiles for one call");
-    CUtensorMap mapDy{}, mapQ{};
+    CUtensorMap mapDy{}, mapQ{}, mapDw{};
+    if (g.dwTma)
+        mapDw = tensorMap2d(g.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.n, g.k, g.dwStride, 32, 32);
     if constexpr (TMA) {
         const auto t = type == TCC_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == TCC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -678,7 +757,7 @@ void launchTiles(const GradArgs& g, const Plan& p, int type, cudaStream_t stream
     attr.val.clusterDim.x = CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    checkCudaCall(cudaLaunchKernelEx(&config, kernel, mapDy, mapQ, g));
+    checkCudaCall(cudaLaunchKernelEx(&config, kernel, mapDy, mapQ, mapDw, g));
     if (p.splits > 1) {
         sumPartials<CG><<<p.tilesN * p.tilesK * CG * (128 * 256 / 4 / 32), 256, 0, stream>>>(g, p.splits);
         checkCudaCall(cudaGetLastError());
@@ -737,7 +816,12 @@ int tcc_weight_grad_int8(const void* grad_y, int type, uint64_t grad_y_stride, c
         g.rows = rows, g.n = n, g.k = k;
         g.tilesN = p.tilesN, g.tilesK = p.tilesK, g.rowsPerSplit = p.rowsPerSplit;
         g.accumulate = accumulate != 0;
-        g.dwVector = rowsAlignedTo(grad_w, grad_w_stride * 4, 16);
+        const uint64_t dyBytes = grad_y_stride * typeBytes(type);
+        g.dyAlign = rowsAlignedTo(grad_y, dyBytes, 8) ? 8 : rowsAlignedTo(grad_y, dyBytes, 4) ? 4 : 2;
+        g.qAlign = rowsAlignedTo(q, q_stride, 4) ? 4 : 1;
+        // A TMA store writes whole 16-byte pieces of a row: k has to end one, or the next columns change.
+        g.dwTma = rowsAlignedTo(grad_w, grad_w_stride * 4, 16) && k % 4 == 0 && grad_w_stride < (1ull << 38) &&
+                  std::max(n, k) <= 0x7FFFFF00u;
         const bool tma = rows != 0 && rowsAlignedTo(grad_y, grad_y_stride * typeBytes(type), 16) &&
                          rowsAlignedTo(q, q_stride, 16) && grad_y_stride < (1ull << 38) && q_stride < (1ull << 40) &&
                          std::max({rows, n, k}) <= 0x7FFFFF00u; // coordinates of a copy are signed

@@ -150,15 +150,17 @@ def test_product_blocks_and_types(m, a_kind, b_kind, a_rows, b_rows):
     check_product(y, want, size, 520)
 
 
-@pytest.mark.parametrize("m", [3, 30, 260])
-def test_product_writes_its_rows_only(m):
-    n, k = 200, 256
-    a, sa, b, sb, want, size = product_case(m, n, k, seed=9)
-    for dtype in (torch.float32, torch.bfloat16):
-        for stride, offset in ((n + 8, 8), (n + 1, 3)):
-            whole = torch.full((m + 2, stride), 7.0, device="cuda", dtype=dtype)
+@pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("n", [200, 201, 203, 1])
+@pytest.mark.parametrize("m", [1, 3, 30, 260])
+def test_product_writes_its_rows_only(m, n, layout):
+    k = 256
+    a, sa, b, sb, want, size = product_case(m, n, k, seed=9, layout=layout)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for stride, offset in (((n + 15) // 8 * 8, 8), (n + 1, 3)):
+            whole = torch.full((m + 3, stride), 7.0, device="cuda", dtype=dtype)
             y = whole.view(-1)[offset + stride:offset + stride + m * stride].view(m, stride)[:, :n]
-            T.matmul_fp8_blocks(a, sa, b, sb, y)
+            T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
             check_product(y, want, size, k)
             left = whole.clone().view(-1)
             left[offset + stride:offset + stride + m * stride].view(m, stride)[:, :n] = 7.0
@@ -283,24 +285,26 @@ def test_backward_against_differences(kind):
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (1, 128, 128), (31, 16, 64), (64, 128, 256), (65, 130, 129), (200, 100, 1000),
                                       (1000, 256, 384), (5000, 48, 130), (333, 520, 264)])
-@pytest.mark.parametrize("aligned", [True, False])
-def test_weight_grad(rows, n, k, dtype, aligned):
+@pytest.mark.parametrize("pad", [0, 1, 2, 4, 8])  # elements that rows lie off a multiple of 16
+def test_weight_grad(rows, n, k, dtype, pad):
     dt = D.TYPES[dtype]
     q64, scales = D.quantize(D.make(rows, k, torch.float32, rows + k), "int8")
-    q = D.strided(rows, k, torch.int8, D.up16(k) if aligned else k + 1, 0 if aligned else 1)
+    q = D.strided(rows, k, torch.int8, D.up16(k) + pad, pad)
     q.copy_(q64.to(torch.int8))
-    dy = D.strided(rows, n, dt, D.up16(n) if aligned else n + 1, 0 if aligned else 1)
+    dy = D.strided(rows, n, dt, D.up16(n) + pad, pad)
     dy.copy_(D.make(rows, n, dt, 5, scale=0.01))
     xv = D.values(q, scales)
     want, size = dy.double().t() @ xv, dy.double().abs().t() @ xv.abs()
     for accumulate in (False, True):
-        start = torch.randn(n, k + 4, device="cuda")[:, :k]
-        dw = start.clone() if not accumulate else torch.zeros(n, k + 4, device="cuda")[:, :k].copy_(start)
+        width = (k + 3) // 4 * 4 + (0 if pad in (0, 2) else 1)  # rows of dw on 16 bytes, or not
+        start = torch.randn(n, width, generator=torch.Generator().manual_seed(rows))[:, :k].cuda()
+        dw = torch.full((n, width), 7.0, device="cuda")[:, :k].copy_(start)
         T.weight_grad_int8(dy, q, scales, dw, accumulate=accumulate)
         target = want + (start.double() if accumulate else 0)
         limit = (rows + 8) * D.U * (size + (start.double().abs() if accumulate else 0)) + 2.0 ** -140
         off = (dw.double() - target).abs()
         assert (off <= limit).all(), f"{int((off > limit).sum())} outside, worst {float((off / limit).max())}"
+        assert (dw.as_strided((n, width - k), (width, 1), k) == 7.0).all()  # between the rows
     assert T.device_status() == 0
 
 
