@@ -125,13 +125,24 @@ __device__ __forceinline__ uint32_t clusterRank() {
     return r;
 }
 // All threads of the CTAs of the cluster.
+__device__ __forceinline__ void clusterBarrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 template <int CG> __device__ __forceinline__ void clusterSync() {
-    if constexpr (CG == 1) {
+    if constexpr (CG == 1)
         __syncthreads();
-    } else {
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    else
+        clusterBarrier();
+}
+// A float at this shared-memory address of another CTA of the cluster.
+__device__ __forceinline__ float ldClusterF32(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
 }
 // Arrive on the barrier at this address of the cluster's first CTA. No cluster-wide release, which
 // took about 1300 cycles and held the MMAs up: nothing that one CTA wrote is read by the other. Each

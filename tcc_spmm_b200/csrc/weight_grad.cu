@@ -351,21 +351,21 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
             if (lane == 0)
                 arriveLeader<CG>(accEmpty);
         }
-        const uint32_t row = n0 + 32 * quarter + laneColumn(lane);
         if (ok && p.partials != nullptr) {
             float4* out = reinterpret_cast<float4*>(p.partials) + uint64_t(blockIdx.x) * (128 * L::kBk / 4) + half * 32 * 128 +
                           32 * quarter + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 out[128 * i] = make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
-        } else if (ok && p.dwTma) {
-            // Boxes of 32 x 32 through the raw ring, which nothing uses any more, swizzled as the map says;
-            // accumulate adds them where they go.
+        } else if (ok) {
+            // Boxes of 32 x 32 through the raw ring, which nothing uses any more, swizzled as the map says:
+            // by TMA, which adds them where they go for accumulate, or, where rows do not start and end on
+            // 16 bytes, row by row with neighbouring lanes on neighbouring columns.
             const uint32_t buf = base + L::kRawOff + warp * 4096, r = laneColumn(lane);
 #pragma unroll
             for (int box = 0; box < 4; ++box) {
                 const uint32_t x = k0 + 128 * half + 32 * box, y = n0 + 32 * quarter;
-                if (lane == 0)
+                if (p.dwTma && lane == 0)
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
 #pragma unroll
@@ -375,32 +375,33 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                                  "f"(sum[32 * box + 4 * j + 1]), "f"(sum[32 * box + 4 * j + 2]),
                                  "f"(sum[32 * box + 4 * j + 3])
                                  : "memory");
-                dev::fenceProxyAsyncShared();
-                __syncwarp();
-                if (lane == 0 && x < p.k && y < p.n) {
-                    if (p.accumulate)
-                        asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
-                                     ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
-                                     : "memory");
-                    else
-                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-                                     ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
-                                     : "memory");
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                if (p.dwTma) {
+                    dev::fenceProxyAsyncShared();
+                    __syncwarp();
+                    if (lane == 0 && x < p.k && y < p.n) {
+                        if (p.accumulate)
+                            asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
+                                         : "memory");
+                        else
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(&mapDw), "r"(x), "r"(y), "r"(buf)
+                                         : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    __syncwarp();
+                    if (x + lane < p.k)
+                        for (uint32_t i = 0; i < 32 && y + i < p.n; ++i) {
+                            float* out = p.dw + uint64_t(y + i) * p.dwStride + x + lane;
+                            const float v = __uint_as_float(dev::ldsU32(buf + i * 128 + (((lane / 4) ^ i) & 7) * 16 + lane % 4 * 4));
+                            *out = v + (p.accumulate ? *out : 0.0f);
+                        }
                 }
             }
-            if (lane == 0) // shared memory stays until the copies have read it
+            if (p.dwTma && lane == 0) // shared memory stays until the copies have read it
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
-        } else if (ok && row < p.n) {
-#pragma unroll
-            for (int i = 0; i < 128; ++i) {
-                const uint32_t col = k0 + 128 * half + i;
-                if (col < p.k) {
-                    float* out = p.dw + row * p.dwStride + col;
-                    *out = sum[i] + (p.accumulate ? *out : 0.0f);
-                }
-            }
         }
     } else if (warp < L::kBWarp) {
         registersDown<L::kRegsA>();

@@ -127,7 +127,7 @@ def test_product(m, n, k, out, layout, aligned):
 
 @pytest.mark.parametrize("layout", ["nk", "kn"])
 @pytest.mark.parametrize("m,n,k", [(2500, 2100, 200), (2500, 1000, 300), (1000, 1217, 640), (9000, 128, 1152), (40000, 260, 128),
-                                   (20, 9000, 136), (700, 4000, 1030)])
+                                   (20, 9000, 136), (700, 4000, 1030), (2500, 2100, 2200), (2500, 1000, 2500), (1000, 1217, 4200)])
 def test_product_many_tiles(m, n, k, layout):
     """More output tiles than SMs, so that a CTA computes several in turn, at every width of tile; several times,
     and with every width of output (a CTA reuses its output buffers while copies read them)."""
@@ -137,6 +137,25 @@ def test_product_many_tiles(m, n, k, layout):
             y = torch.full((m, n), float("nan"), device="cuda", dtype=dtype)
             T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
             check_product(y, want, size, k)
+    assert T.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("m,n,k", [(20, 130, 1024), (100, 500, 2100), (40, 64, 4300), (130, 1000, 8192), (600, 900, 1500),
+                                   (17, 2000, 3333), (256, 4096, 1152)])
+def test_product_split(m, n, k, layout):
+    """Few output tiles and a long k, which several CTAs share."""
+    a, sa, b, sb, want, size = product_case(m, n, k, layout=layout, seed=m)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(k)).cuda()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for stride in (n, D.up16(n) + 16):
+            y = torch.full((m, stride), float("nan"), device="cuda", dtype=dtype)
+            T.matmul_fp8_blocks(a, sa, b, sb, y[:, :n], bias=bias, b_layout=layout)
+            check_product(y[:, :n], want, size, k, bias)
+            assert y[:, n:].isnan().all()
+            again = torch.empty(m, n, device="cuda", dtype=dtype)
+            T.matmul_fp8_blocks(a, sa, b, sb, again, bias=bias, b_layout=layout)
+            assert torch.equal(again, y[:, :n])
     assert T.device_status() == 0
 
 
@@ -495,6 +514,37 @@ def test_layer_against_64_bits():
     kept = D.values(s["kept"], s["kept_s"])
     size = s["dz"].double().abs().t() @ kept.abs()
     assert ((s["dw"].double() - s["dz"].double().t() @ kept).abs() <= (m + 8) * D.U * size).all()
+
+
+@pytest.mark.parametrize("features", [128, 256])
+def test_graph_layer(features):
+    """A graph layer and its weight gradient: the aggregated features (the SpMM's fp32 output) quantized and
+    multiplied by the layer's weights, kept for the backward pass as well."""
+    from tests.cases import EDGE_CASES
+    from tests.gpu_util import build_case, run_spmm
+
+    y = run_spmm(build_case(EDGE_CASES["random_local"](), features, seed=3))
+    rows, n = y.shape[0], 96
+    q = torch.empty(rows, features, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.empty(rows, features // 128, dtype=torch.uint8, device="cuda")
+    T.quantize_blocks_fp8(y, q, scales)
+    kept, kept_s = torch.empty(rows, features, dtype=torch.int8, device="cuda"), torch.empty_like(scales)
+    T.activation_checkpoint_int8(y, None, kept, kept_s, activation="identity")
+    w64, ws = D.quantize(D.make(n, features, torch.float32, 8, scale=0.1), "e4m3", 128)
+    w = w64.float().to(torch.float8_e4m3fn)
+    z = torch.empty(rows, n, device="cuda")
+    T.matmul_fp8_blocks(q, scales, w, ws, z)
+    for got, got_s, kind in ((q, scales, "e4m3"), (kept, kept_s, "int8")):
+        want, bytes_ = D.quantize(y, kind)
+        assert torch.equal(got_s, bytes_) and same(got, want)
+    yv, wv = D.values(q, scales), D.values(w, ws, 128)
+    check_product(z, yv @ wv.t(), yv.abs() @ wv.abs().t(), features)
+    grad = D.make(rows, n, torch.float32, 9, scale=0.01)
+    dw = torch.empty(n, features, device="cuda")
+    T.weight_grad_int8(grad, kept, kept_s, dw)
+    kv = D.values(kept, kept_s)
+    limit = (rows + 8) * D.U * (grad.double().abs().t() @ kv.abs())
+    assert ((dw.double() - grad.double().t() @ kv).abs() <= limit).all()
 
 
 def test_streams_and_graph():
