@@ -308,8 +308,8 @@ int tcc_spmm_launch_shape(uint32_t features, int variant, uint32_t* grid, uint32
  * byte 255 (NaN) and elements NaN (INT8: 0), and all that is computed from it is NaN.
  *
  * Strides are row strides in elements, at least the row's width; elements of a row are adjacent.
- * A size of 0 is allowed. The matrices of a call must not overlap, but for y == x and
- * grad_x == grad_y with equal strides.
+ * Sizes from 0 to 2^32 - 256 are allowed. The matrices of a call must not overlap, but for y == x
+ * and grad_x == grad_y with equal strides.
  * --------------------------------------------------------------------------------- */
 
 typedef enum tcc_type { TCC_F32 = 0, TCC_BF16 = 1, TCC_F16 = 2, TCC_E4M3 = 3, TCC_E5M2 = 4 } tcc_type;

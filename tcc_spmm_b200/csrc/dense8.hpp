@@ -26,9 +26,12 @@ inline bool isFloatType(int t) { return t == TCC_F32 || t == TCC_BF16 || t == TC
 inline bool isFp8Type(int t) { return t == TCC_E4M3 || t == TCC_E5M2; }
 inline uint32_t typeBytes(int t) { return t == TCC_F32 ? 4 : (t == TCC_BF16 || t == TCC_F16) ? 2 : 1; }
 template <typename T> T ceilDiv(T a, T b) { return (a + b - 1) / b; }
-// The matrix's bytes do not reach over the end of the address space (rows, cols > 0).
+// The largest number of rows or columns: sizes are rounded up to whole tiles of up to 256 in 32 bits.
+constexpr uint32_t kLargestSize = 0xFFFFFF00u;
+// The matrix's bytes do not reach over the end of the address space, nor its sizes over kLargestSize
+// (rows, cols > 0).
 inline bool extentFits(uint64_t rows, uint64_t cols, uint64_t stride, uint64_t elementBytes) {
-    return stride <= (uint64_t(1) << 60) / elementBytes / rows && cols <= stride;
+    return rows <= kLargestSize && cols <= kLargestSize && stride <= (uint64_t(1) << 60) / elementBytes / rows && cols <= stride;
 }
 inline int currentDevice() {
     int device = 0;

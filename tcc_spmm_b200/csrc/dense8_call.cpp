@@ -27,9 +27,11 @@ extern "C" int tcc_dense8_call(int op, const uint64_t* v) {
         return tcc_activation_backward_int8(ptr<void>(v[0]), v[1], i32(v[2]), ptr<int8_t>(v[3]), v[4], ptr<uint8_t>(v[5]),
                                             ptr<void>(v[6]), v[7], u32(v[8]), u32(v[9]), i32(v[10]),
                                             ptr<CUstream_st>(v[11]));
-    default:
+    case 4:
         return tcc_weight_grad_int8(ptr<void>(v[0]), i32(v[1]), v[2], ptr<int8_t>(v[3]), v[4], ptr<uint8_t>(v[5]),
                                     ptr<float>(v[6]), v[7], u32(v[8]), u32(v[9]), u32(v[10]), i32(v[11]),
                                     ptr<void>(v[12]), v[13], ptr<CUstream_st>(v[14]));
+    default:
+        return TCC_INVALID_ARGUMENT;
     }
 }

@@ -6,7 +6,7 @@ power-of-two scale, kept as its biased exponent byte (torch.uint8, or torch.floa
 2^(byte - 127)). include/tcc_spmm_b200.h states the rule.
 
 Every operand is a 2-D CUDA tensor of one device whose last dimension has stride 1; rows may be
-any distance apart. The calls enqueue work on `stream` (default: torch's current stream of that
+any distance apart, and the tensors of a call share no memory but where it says so. The calls enqueue work on `stream` (default: torch's current stream of that
 device), never synchronise, and raise InvalidArgument for tensors that do not fit together. They
 write into tensors that the caller gives. The reference has no counterpart.
 
@@ -26,6 +26,7 @@ from .api import InvalidArgument, _check, _stream_handle
 BLOCK = 128
 ACTIVATIONS = {"relu": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "identity": 4}
 LAYOUTS = {"nk": 0, "kn": 1}
+_LARGEST = 0xFFFFFF00  # rows or columns: the kernels round them up to whole tiles in 32 bits
 
 # torch, its raw-stream and current-device queries, and the type codes, once an operator is used
 _torch = _raw_stream = _current_device = _call = None
@@ -62,7 +63,7 @@ def _matrix(name: str, t, device: int = -1) -> tuple:
         _refuse(f"{name} must be a CUDA tensor")
     if on != device and device >= 0:
         _refuse(f"{name} is on cuda:{on}, expected cuda:{device}")
-    if rows > 0xFFFFFFFF or cols > 0xFFFFFFFF:
+    if rows > _LARGEST or cols > _LARGEST:
         _refuse(f"{name} is too large")
     if col_stride != 1 and cols > 1:
         _refuse(f"{name} must have stride 1 along its last dimension")
@@ -90,6 +91,8 @@ def _shaped(name: str, t, rows: int, cols: int, device: int) -> int:
 def _scales(name: str, t, device: int, rows: int, cols: int, row_blocks: bool = True, square_blocks: bool = True) -> int:
     """Checks the scale bytes of a [rows, cols] matrix and returns the rows per block."""
     wide = (cols + 127) >> 7
+    if not isinstance(t, _torch.Tensor):
+        _refuse(f"{name} must be a CUDA tensor")
     if t.dtype in _SCALES and t.get_device() == device and t.is_contiguous():
         shape = t.shape
         if row_blocks and shape == (rows, wide):
@@ -168,8 +171,8 @@ def matmul_fp8_blocks(a, a_scales, b, b_scales, output, bias=None, b_layout: str
     at, bt, ot = _type("a", a, _FP8), _type("b", b, _FP8), _type("output", output, _FLOATS)
     a_block = _scales("a_scales", a_scales, device, m, k)
     b_block = _scales("b_scales", b_scales, device, b_rows, b_cols, not layout)
-    if bias is not None and not (bias.dtype == _torch.float32 and tuple(bias.shape) == (n,) and bias.is_contiguous() and
-                                 bias.get_device() == device):
+    if bias is not None and not (isinstance(bias, _torch.Tensor) and bias.dtype == _torch.float32 and tuple(bias.shape) == (n,) and
+                                 bias.is_contiguous() and bias.get_device() == device):
         _refuse(f"bias must be {n} contiguous fp32 values on cuda:{device}")
     _launch(device, stream, _PRODUCT, a.data_ptr(), at, as_, a_scales.data_ptr(), a_block,
             b.data_ptr(), bt, bs, b_scales.data_ptr(), b_block, layout, 0 if bias is None else bias.data_ptr(),
@@ -237,6 +240,8 @@ def activation_backward_int8(grad_y, q, scales, grad_x, activation: str = "gelu"
 
 def weight_grad_int8_workspace_size(rows: int, n: int, k: int) -> int:
     """Bytes of workspace that weight_grad_int8 needs for grad_y [rows, n] and a checkpoint [rows, k]."""
+    if not all(0 <= size <= _LARGEST for size in (rows, n, k)):
+        _refuse(f"rows, n and k must be between 0 and {_LARGEST}")
     size = C.c_uint64()
     _check(N.lib().tcc_weight_grad_int8_workspace_size(rows, n, k, C.byref(size)))
     return size.value
@@ -272,7 +277,8 @@ def weight_grad_int8(grad_y, q, scales, grad_w, accumulate: bool = False, worksp
                 stream = cuda.ExternalStream(stream, device) if stream else cuda.default_stream(device)
             with _torch.cuda.stream(stream):  # nothing for None: the current stream
                 workspace = _torch.empty(need, dtype=_torch.uint8, device=grad_y.device)
-    elif workspace.get_device() != device or not workspace.is_contiguous():
+    elif (not isinstance(workspace, _torch.Tensor) or workspace.get_device() != device or
+          not workspace.is_contiguous()):
         _refuse(f"the workspace must be contiguous on cuda:{device}")
     have = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _launch(device, stream, _WEIGHT_GRAD, grad_y.data_ptr(), gt, gs, q.data_ptr(), qs,

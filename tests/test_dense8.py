@@ -62,6 +62,38 @@ def test_c_abi_refuses_before_any_device_work(native):
     assert native.tcc_weight_grad_int8_workspace_size(4, 0, 128, C.byref(size)) == 0 and size.value == 0
 
 
+def test_c_abi_refuses_sizes_that_no_tile_count_holds(native):
+    """Sizes are rounded up to whole blocks and tiles of up to 256 in 32 bits."""
+    size, big, wide = C.c_uint64(), 0xFFFFFF01, 1 << 32
+    quantize, product, grad = native.tcc_quantize_blocks_fp8, native.tcc_matmul_fp8_blocks, native.tcc_weight_grad_int8
+    keep, back = native.tcc_activation_checkpoint_int8, native.tcc_activation_backward_int8
+    bad = [
+        (quantize, (16, 0, wide, 16, 3, wide, 16, 1, big, 1, None)),
+        (quantize, (16, 0, 1, 16, 3, 1, 16, big, 1, 128, None)),
+        (keep, (16, wide, 16, wide, 0, 16, wide, 16, 1, 0xFFFFFFFF, 1, None)),
+        (back, (16, wide, 0, 16, wide, 16, 16, wide, 1, 0xFFFFFFFF, 1, None)),
+        (product, (16, 3, 1, 16, 1, 16, 3, 1, 16, 128, 0, None, 16, 0, 1, big, 1, 1, None)),
+        (product, (16, 3, 1, 16, 1, 16, 3, 1, 16, 128, 0, None, 16, 0, wide, 1, big, 1, None)),
+        (product, (16, 3, wide, 16, 1, 16, 3, wide, 16, 128, 0, None, 16, 0, 1, 1, 1, big, None)),
+        (grad, (16, 0, 1, 16, 1, 16, 16, 1, 0xFFFFFFFF, 1, 1, 0, 16, 1 << 40, None)),
+        (grad, (16, 0, 1, 16, wide, 16, 16, wide, 1, 1, big, 0, 16, 1 << 40, None)),
+        (native.tcc_weight_grad_int8_workspace_size, (big, 128, 128, C.byref(size))),
+        (native.tcc_weight_grad_int8_workspace_size, (128, 128, big, C.byref(size))),
+    ]
+    for call, args in bad:
+        assert call(*args) == 1, (call.__name__, args)
+        assert b"too large" in native.tcc_last_error(), (call.__name__, args, native.tcc_last_error())
+    assert native.tcc_weight_grad_int8_workspace_size(0xFFFFFF00, 128, 128, C.byref(size)) == 0
+    for sizes in ((-1, 128, 128), (1 << 32, 128, 128), (128, 128, big)):
+        with pytest.raises(T.InvalidArgument):
+            T.weight_grad_int8_workspace_size(*sizes)
+
+
+def test_packed_call_refuses_unknown_operators(native):
+    for op in (-1, 5):
+        assert native.tcc_dense8_call(op, bytes(8 * 19)) == 1
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros(4, 128)
     q = torch.zeros(4, 128, dtype=torch.int8)

@@ -448,6 +448,29 @@ def test_refusals():
             pytest.fail(f"call {i} was not refused")
 
 
+def test_refuses_what_is_no_tensor():
+    x = torch.zeros(8, 256, device="cuda")
+    q = torch.zeros(8, 256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.full((8, 2), 127, dtype=torch.uint8, device="cuda")
+    i8 = torch.zeros(8, 256, dtype=torch.int8, device="cuda")
+    dw = torch.zeros(256, 256, device="cuda")
+    bad = [
+        lambda: T.quantize_blocks_fp8(x, q, None),
+        lambda: T.quantize_blocks_fp8([[1.0]], q, s),
+        lambda: T.quantize_blocks_fp8(x, None, s),
+        lambda: T.matmul_fp8_blocks(q, None, q, s, x[:, :8]),
+        lambda: T.matmul_fp8_blocks(q, s, q, s, x[:, :8], bias=[0.0] * 8),
+        lambda: T.activation_checkpoint_int8(x, None, i8, s),
+        lambda: T.activation_checkpoint_int8(x, x.clone(), i8, 127),
+        lambda: T.activation_backward_int8(x, i8, s, None),
+        lambda: T.weight_grad_int8(x, i8, None, dw),
+        lambda: T.weight_grad_int8(x, i8, s, dw, workspace=1 << 20),
+    ]
+    for call in bad:
+        with pytest.raises(T.InvalidArgument):
+            call()
+
+
 # ---- streams and graphs -------------------------------------------------------------------------------
 def layer(x, w, ws, grad, bias, stages=False):
     """One layer forward and backward, as a training step runs it: quantize, product, activation with its input
