@@ -34,6 +34,7 @@ __device__ __forceinline__ float fp8Value(uint8_t v, bool e4m3) {
 // ---- any strides and alignment ----------------------------------------------------------------
 // 64 x 64 outputs per CTA, 4 x 4 per thread, FP32 FMA from operands dequantized into shared memory.
 // For matrices whose rows do not start on 16 bytes, which the tensor-core kernels' copies cannot read.
+// FMA and shared-memory bound: 21 TFLOP/s at 8192 x 4096 x 4096.
 constexpr int kTile = 64, kStep = 32;
 
 template <typename T>
@@ -104,7 +105,8 @@ template <typename T> void launchGeneric(const Product& p) {
 // all of a 4096-wide row in flight at once), and their sums are added up in shared memory at the end, in
 // a fixed order. The order of k in mma.m16n8k32 may be any that both operands share, so a lane reads 16
 // bytes of k of two rows of b and of MT rows of a at a time: two MMAs per 64 of k and 8 rows of a. The sum
-// over a block is multiplied by the two scales' product, a power of two.
+// over a block is multiplied by the two scales' product, a power of two. 7.2 us for 1 x 4096 x 4096 out of
+// HBM (2.3 TB/s; 2.4 us of it launch and drain), 20.9 us for 1 x 8192 x 8192 (3.2 TB/s).
 template <int MT_> struct Few {
     static constexpr int MT = MT_;
     static constexpr int kWarps = 8, kRows = 16;         // rows of b per CTA
@@ -267,6 +269,10 @@ template <int MT> void launchFew(const Product& p) {
 // consecutive blocks per row, loaded by warps of their own, copied to tensor memory by the MMA thread
 // and picked by the byte selector of the instruction descriptor. Eight warps bring finished tiles into
 // registers, release the accumulator, and write them by TMA through 4 KB of shared memory each.
+//
+// Large products run at the power limit: 8192 x 4096 x 4096 bf16 takes 93 us (2.95 PFLOP/s) on operands of
+// few distinct exponents and 116 to 124 us on normal ones, 8192^3 351 us (3.13 PFLOP/s). Few columns are
+// bound by HBM: 1M x 128 x 256 fp32 149 us (5.4 TB/s), bf16 90 us (5.9 TB/s).
 template <int BN_, int CG_> struct Tile {
     static constexpr int BN = BN_, CG = CG_;
     static constexpr int kStages = BN == 256 ? 5 : BN == 128 ? 4 : 6;
