@@ -272,7 +272,7 @@ template <int MT> void launchFew(const Product& p) {
 //
 // Large products run at the power limit: 8192 x 4096 x 4096 bf16 takes 93 us (2.95 PFLOP/s) on operands of
 // few distinct exponents and 116 to 124 us on normal ones, 8192^3 351 us (3.13 PFLOP/s). Few columns are
-// bound by HBM: 1M x 128 x 256 fp32 149 us (5.4 TB/s), bf16 90 us (5.9 TB/s).
+// bound by HBM: 1M x 128 x 256 fp32 145 us (5.5 TB/s), bf16 88 us (6.1 TB/s).
 template <int BN_, int CG_> struct Tile {
     static constexpr int BN = BN_, CG = CG_;
     static constexpr int kStages = BN == 256 ? 5 : BN == 128 ? 4 : 6;
@@ -324,7 +324,10 @@ struct ProductArgs {
     void* out;
     uint64_t outStride;
     int outType;
-    bool outTma; // output rows start and end on 16 bytes: written by TMA
+    bool outTma;   // output rows start and end on 16 bytes: written by TMA
+    bool outWords; // output rows start and end on 4 bytes
+    uint32_t aBytes, bBytes; // what a stage's two copies bring
+    bool keepB; // one column of tiles, and a stage always holds the same block of k: its b stays
     uint32_t m, n, k, tilesM, tilesN;
     uint32_t idesc;
     uint32_t splits, splitBlocks; // of SPLIT: CTAs per tile (2, 4 or 8), blocks of k each (a multiple of 4)
@@ -388,6 +391,43 @@ template <int LEFT> __device__ __forceinline__ void tmaStoreWaitRead() {
     asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
 }
 
+// Up to 32 rows of a box of WIDTH bytes a row to the output, `bytes` of each, in pieces of W bytes:
+// neighbouring lanes on neighbouring pieces, several rounds of loads before their stores (701999 x 21 x 256 fp32
+// 93 -> 46 us).
+template <int WIDTH, int W>
+__device__ __forceinline__ void copyRows(uint32_t at, void* out, uint64_t step, uint32_t rows, uint32_t bytes, uint32_t lane) {
+    constexpr uint32_t kLanes = WIDTH / W < 32 ? WIDTH / W : 32, kRows = 32 / kLanes, kPieces = WIDTH / W / kLanes;
+    constexpr uint32_t kBatch = kRows > 4 ? 32 / kRows : 8 / kPieces;
+    static_assert(32 % (kRows * kBatch) == 0, "rounds end with the box");
+    const uint32_t sub = lane / kLanes, byte0 = lane % kLanes * W;
+    uint8_t* to = static_cast<uint8_t*>(out) + sub * step + byte0;
+    for (uint32_t row0 = 0; row0 < rows; row0 += kRows * kBatch) {
+        uint32_t v[kBatch][kPieces];
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b)
+#pragma unroll
+            for (uint32_t i = 0; i < kPieces; ++i) {
+                const uint32_t row = row0 + b * kRows + sub, byte = byte0 + i * kLanes * W;
+                const uint32_t piece = WIDTH == 128 ? (byte / 16) ^ (row & 7) : byte / 16;
+                const uint32_t from = at + row * WIDTH + piece * 16 + byte % 16;
+                if constexpr (W == 4)
+                    v[b][i] = dev::ldsU32(from);
+                else
+                    asm volatile("{ .reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t; }" : "=r"(v[b][i]) : "r"(from) : "memory");
+            }
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b, to += kRows * step)
+#pragma unroll
+            for (uint32_t i = 0; i < kPieces; ++i)
+                if (row0 + b * kRows + sub < rows && byte0 + i * kLanes * W < bytes) {
+                    if constexpr (W == 4)
+                        *reinterpret_cast<uint32_t*>(to + i * kLanes * W) = v[b][i];
+                    else
+                        *reinterpret_cast<unsigned short*>(to + i * kLanes * W) = static_cast<unsigned short>(v[b][i]);
+                }
+    }
+}
+
 // One warp's 32 rows x kHalf columns of a finished tile: lane = row. Boxes of 32 rows x 128 bytes (or
 // the whole width, if less) go through shared memory, swizzled as the map says, to the output by TMA, or,
 // where rows do not start and end on 16 bytes, row by row with neighbouring lanes on neighbouring
@@ -422,25 +462,13 @@ __device__ __forceinline__ void storeTile(const ProductArgs& p, const CUtensorMa
                 tmaStore2d(map, at, c0, uint32_t(row0));
         } else {
             __syncwarp();
-            const uint32_t rows = uint32_t(min(uint64_t(32), p.m - row0)), cols = min(uint32_t(kPerBox), p.n - c0);
+            const uint32_t rows = uint32_t(min(uint64_t(32), p.m - row0));
+            const uint32_t bytes = min(uint32_t(kPerBox), p.n - c0) * uint32_t(sizeof(T));
             T* out = static_cast<T*>(p.out) + row0 * p.outStride + c0;
-#pragma unroll 4
-            for (uint32_t row = 0; row < rows; ++row, out += p.outStride)
-#pragma unroll
-                for (uint32_t c = lane; c < uint32_t(kPerBox); c += 32) {
-                    const uint32_t byte = c * uint32_t(sizeof(T));
-                    const uint32_t piece = kWidth == 128 ? (byte / 16) ^ (row & 7) : byte / 16;
-                    const uint32_t from = at + row * kWidth + piece * 16 + byte % 16;
-                    if (c < cols) {
-                        if constexpr (sizeof(T) == 4) {
-                            reinterpret_cast<uint32_t*>(out)[c] = dev::ldsU32(from);
-                        } else {
-                            unsigned short v;
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-                            reinterpret_cast<unsigned short*>(out)[c] = v;
-                        }
-                    }
-                }
+            if (sizeof(T) == 4 || p.outWords)
+                copyRows<kWidth, 4>(at, out, p.outStride * sizeof(T), rows, bytes, lane);
+            else
+                copyRows<kWidth, 2>(at, out, p.outStride * sizeof(T), rows, bytes, lane);
         }
     }
 }
@@ -524,9 +552,12 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                         break;
                     }
                     const uint32_t a = base + stage * L::kStageBytes, b = a + L::kABytes, bar = full + 8 * stage;
-                    dev::mbarArriveExpectTx(bar, L::kStageBytes);
+                    const bool bringB = !p.keepB || it < L::kStages;
+                    dev::mbarArriveExpectTx(bar, p.aBytes + (bringB ? p.bBytes : 0u));
                     tmaLoad2d(a, &mapA, kb * kBlock, uint32_t(m0), bar);
-                    if constexpr (KN)
+                    if (!bringB)
+                        ;
+                    else if constexpr (KN)
                         tmaLoad2d(b, &mapB, n0, kb * kBlock, bar);
                     else
                         tmaLoad2d(b, &mapB, kb * kBlock, n0, bar);
@@ -792,15 +823,23 @@ template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Pr
     args.outType = p.outType;
     // A TMA store writes whole 16-byte pieces of a row: n has to end one, or the next columns change.
     args.outTma = rowsAlignedTo(p.out, p.outStride * outBytes, 16) && p.n * uint64_t(outBytes) % 16 == 0 && p.outStride < (1ull << 38);
+    args.outWords = rowsAlignedTo(p.out, p.outStride * outBytes, 4) && p.n * uint64_t(outBytes) % 4 == 0;
     args.m = p.m, args.n = p.n, args.k = p.k;
     args.tilesM = ceilDiv<uint32_t>(p.m, 128 * CG);
     args.tilesN = ceilDiv<uint32_t>(p.n, BN);
     require(uint64_t(args.tilesM) * args.tilesN <= 0x3FFFFFFFull, "too many output tiles for one call");
     args.idesc = scaledIdesc(p.a.type == TCC_E5M2, p.b.type == TCC_E5M2, KN, 128 * CG, BN);
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUtensorMap mapA = tensorMap2d(p.a.data, u8, 1, p.m, p.k, p.a.stride, 128, 128);
+    // A box ends with a matrix of fewer rows than a tile: filling rows up with zeros takes a copy longer than
+    // loading them (17 x 4096 x 4096 17.2 -> 11.2 us), and what is left in their place only reaches outputs
+    // that are not there.
+    const uint32_t aRows = std::min(128u, p.m), bRows = KN ? 128u : std::min<uint32_t>(L::kBRows, p.n);
+    args.aBytes = aRows * 128, args.bBytes = bRows * 128;
+    // 701999 x 21 x 65 fp32 72 -> 48 us, 1M x 128 x 256 fp32 149 -> 145 us.
+    args.keepB = args.tilesN == 1 && L::kStages % kBlocks == 0;
+    const CUtensorMap mapA = tensorMap2d(p.a.data, u8, 1, p.m, p.k, p.a.stride, aRows, 128);
     const CUtensorMap mapB = KN ? tensorMap2d(p.b.data, u8, 1, p.k, p.n, p.b.stride, 128, 128)
-                                : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, L::kBRows, 128);
+                                : tensorMap2d(p.b.data, u8, 1, p.n, p.k, p.b.stride, bRows, 128);
     CUtensorMap mapOut{};
     if (args.outTma) {
         const uint32_t width = std::min<uint32_t>(128, L::kHalf * outBytes);
@@ -808,7 +847,7 @@ template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Pr
                              p.outType == TCC_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                              : p.outType == TCC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                             outBytes, p.m, p.n, p.outStride, 32, width / outBytes,
+                             outBytes, p.m, p.n, p.outStride, std::min(32u, p.m), width / outBytes,
                              width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
     }
     args.splits = splits;
@@ -865,7 +904,13 @@ void launchProduct(const Product& p) {
         p.kn ? launchTiles<128, 1, true, true>(p, splits) : launchTiles<128, 1, false, true>(p, splits);
         return;
     }
-    if (p.n > 128 && ceilDiv(p.m, 256u) * uint64_t(ceilDiv(p.n, 256u)) * 2 >= sms)
+    // The narrowest tile that holds n (701999 x 24 x 128 fp32 39 -> 35 us); of wider n the widest tile
+    // that leaves few SMs idle.
+    if (!p.kn && p.n <= 32)
+        launchTiles<32, 1, false>(p);
+    else if (!p.kn && p.n <= 64)
+        launchTiles<64, 1, false>(p);
+    else if (p.n > 128 && ceilDiv(p.m, 256u) * uint64_t(ceilDiv(p.n, 256u)) * 2 >= sms)
         p.kn ? launchTiles<256, 2, true>(p) : launchTiles<256, 2, false>(p);
     else if (p.kn || rowTiles * ceilDiv(p.n, 128u) >= sms)
         p.kn ? launchTiles<128, 1, true>(p) : launchTiles<128, 1, false>(p);

@@ -141,6 +141,21 @@ def test_product_many_tiles(m, n, k, layout):
 
 
 @pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("n", [5, 21, 32, 33, 64, 100, 128, 129, 256])
+@pytest.mark.parametrize("k", [1, 65, 128, 256, 300, 500, 640, 700])
+def test_product_tall(n, k, layout):
+    """Few columns and so many rows that a CTA's stages come round several times, with one to six blocks of k; the
+    output's rows end on 16, 4 and 2 bytes."""
+    m = 150001 if n <= 128 else 400001
+    a, sa, b, sb, want, size = product_case(m, n, k, layout=layout, seed=n)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = torch.full((m, n), float("nan"), device="cuda", dtype=dtype)
+        T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
+        check_product(y, want, size, k)
+    assert T.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["nk", "kn"])
 @pytest.mark.parametrize("m,n,k", [(20, 130, 1024), (100, 500, 2100), (40, 64, 4300), (130, 1000, 8192), (600, 900, 1500),
                                    (17, 2000, 3333), (256, 4096, 1152)])
 def test_product_split(m, n, k, layout):
