@@ -220,7 +220,7 @@ inline CUtensorMap tensorMap2d(const void* base, CUtensorMapDataType type, uint3
     const cuuint64_t strides[1] = {stride * elementBytes};
     const cuuint32_t box[2] = {boxCols, boxRows}, steps[2] = {1, 1};
     if (encode(&map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
+               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
         CUDA_SUCCESS)
         throw CudaError("cuTensorMapEncodeTiled refused a matrix");
     return map;
