@@ -392,6 +392,52 @@ def test_weight_grad_not_finite_gradient(dtype):
         assert dw[2].isnan().all()
 
 
+# ---- alignments -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("cols", [1, 3, 50, 64, 127, 130, 255, 300])
+def test_rows_of_any_alignment(kind, cols):
+    """Every pair of alignments of a float matrix and an 8-bit one: the bytes are those of packed copies, nothing
+    beyond a row is written."""
+    rows, dtype = 131, D.TYPES[kind]
+    x = D.make(rows, cols, dtype, cols)
+
+    def place(dtype, stride, offset):
+        whole = torch.full((rows * stride + offset + 16,), 5.0, device="cuda").to(dtype)
+        return whole, whole[offset:offset + rows * stride].view(rows, stride)[:, :cols]
+
+    q0 = torch.empty(rows, D.up16(cols), dtype=torch.int8, device="cuda")[:, :cols]
+    s0 = torch.empty(rows, -(-cols // 128), dtype=torch.uint8, device="cuda")
+    y0, g0 = torch.empty_like(x), torch.empty_like(x)
+    T.activation_checkpoint_int8(x, y0, q0, s0, activation="silu")
+    T.activation_backward_int8(x, q0, s0, g0, activation="silu")
+    want_rows = D.quantize(x, "e4m3", 1)
+    want_squares = D.quantize(x, "e4m3", 128)
+    wide = (cols + 31) // 16 * 16
+    for x_stride, x_offset in ((wide, 0), (wide + 4, 4), (wide + 2, 2), (wide + 1, 1)):
+        xs = place(dtype, x_stride, x_offset)[1]
+        xs.copy_(x)
+        for q_stride, q_offset in ((wide, 0), (wide + 8, 8), (wide + 4, 4), (wide + 2, 2), (wide + 1, 1)):
+            whole_q, q = place(torch.int8, q_stride, q_offset)
+            whole_y, y = place(dtype, x_stride, x_offset)
+            whole_g, g = place(dtype, x_stride, x_offset)
+            s = torch.empty_like(s0)
+            T.activation_checkpoint_int8(xs, y, q, s, activation="silu")
+            assert torch.equal(s, s0) and torch.equal(q, q0) and torch.equal(y, y0)
+            T.activation_backward_int8(xs, q, s, g, activation="silu")
+            assert torch.equal(g, g0)
+            for whole, part in ((whole_q, q), (whole_y, y), (whole_g, g)):
+                part.fill_(5)
+                assert (whole == 5).all()
+            f = q.view(torch.float8_e4m3fn)
+            for block_rows, (want, scales) in ((1, want_rows), (128, want_squares)):
+                got = torch.empty_like(scales)
+                whole_q.fill_(5)
+                T.quantize_blocks_fp8(xs, f, got, block_rows=block_rows)
+                assert torch.equal(got, scales) and torch.equal(f.double(), want)
+                q.fill_(5)
+                assert (whole_q == 5).all()
+
+
 # ---- sizes of zero, refusals ------------------------------------------------------------------------
 def test_empty():
     e4 = torch.float8_e4m3fn
