@@ -651,31 +651,33 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
         tmemDeallocGroup<CG>(tmem, 512);
 }
 
-// dW (+)= the partial tiles, added in the order of their row ranges within eight interleaved sums
-// that are then added in order: the result does not depend on timing. 32 float4 columns of a CTA's
-// partial tile per block, eight threads each.
-template <int CG>
-__global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t splits) {
-    __shared__ float4 sums[8][32];
-    constexpr uint32_t kPerCta = 128 * 256 / 4;
-    const uint64_t item = uint64_t(blockIdx.x) * 32 + threadIdx.x % 32;
+// dW (+)= the partial tiles, added in the order of their row ranges, where there are many within eight
+// interleaved sums that are then added in order: the result does not depend on timing. 256 / PARTS float4
+// columns of a CTA's partial tile per block, PARTS threads each. (8192 x 1024 x 1024 bf16, four ranges: 35
+// -> 26 us for both kernels with PARTS = 1 instead of 8 and stores of 16 bytes.)
+template <int CG, int PARTS> __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t splits) {
+    constexpr uint32_t kPerCta = 128 * 256 / 4, kColumns = 256 / PARTS;
+    const uint64_t item = uint64_t(blockIdx.x) * kColumns + threadIdx.x % kColumns;
     const uint32_t cta = uint32_t(item / kPerCta), within = uint32_t(item % kPerCta);
-    const uint32_t part = threadIdx.x / 32;
+    const uint32_t part = threadIdx.x / kColumns;
     const uint64_t step = uint64_t(p.tilesN) * p.tilesK * CG * kPerCta;
     const float4* in = reinterpret_cast<const float4*>(p.partials) + item;
     float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll 4
-    for (uint32_t s = part; s < splits; s += 8) {
+    for (uint32_t s = part; s < splits; s += PARTS) {
         const float4 v = __ldcs(in + s * step);
         sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
     }
-    sums[part][threadIdx.x % 32] = sum;
-    __syncthreads();
-    if (part != 0)
-        return;
-    for (int i = 1; i < 8; ++i) {
-        const float4 v = sums[i][threadIdx.x];
-        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+    if constexpr (PARTS > 1) {
+        __shared__ float4 sums[PARTS][kColumns];
+        sums[part][threadIdx.x % kColumns] = sum;
+        __syncthreads();
+        if (part != 0)
+            return;
+        for (int i = 1; i < PARTS; ++i) {
+            const float4 v = sums[i][threadIdx.x];
+            sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+        }
     }
     const uint32_t l = within % 128, c = within / 128 * 4, tile = cta / CG;
     const uint32_t row = (tile % p.tilesN * CG + cta % CG) * 128 + l / 32 * 32 + laneColumn(l % 32);
@@ -683,6 +685,15 @@ __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t sp
     if (row >= p.n || col >= p.k)
         return;
     float* out = p.dw + row * p.dwStride + col;
+    if (p.dwTma) { // rows start and end on 16 bytes
+        float4* to = reinterpret_cast<float4*>(out);
+        if (p.accumulate) {
+            const float4 v = *to;
+            sum = make_float4(v.x + sum.x, v.y + sum.y, v.z + sum.z, v.w + sum.w);
+        }
+        *to = sum;
+        return;
+    }
     const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -693,20 +704,21 @@ __global__ void __launch_bounds__(256) sumPartials(const GradArgs p, uint32_t sp
 // How the sum over the rows is split: `splits` ranges of rowsPerSplit rows, one CTA per range and
 // tile of dW. More than one range leaves partial tiles, which sumPartials adds. The number of
 // ranges is the cheapest by an estimate for 148 SMs: waves of CTAs, each row of a range at the MMA
-// rate and each CTA with a fixed start and end, against the partial tiles' traffic.
+// rate and each CTA with a fixed start and end, against the partial tiles' traffic through L2 (2048 x 1024 x
+// 1024 bf16: 22.6 us in one range, 14.7 us in four).
 struct Plan {
     int cg;
     uint32_t tilesN, tilesK, splits, rowsPerSplit;
 };
 Plan planOf(uint32_t rows, uint32_t n, uint32_t k) {
-    constexpr double kSms = 148, kFixedUs = 5, kSumUs = 4;
+    constexpr double kSms = 148, kFixedUs = 5, kSumUs = 3;
     Plan p{};
     p.cg = n <= 128 ? 1 : 2;
     p.tilesN = ceilDiv(n, 128u * p.cg);
     p.tilesK = ceilDiv(k, 256u);
     const double tiles = double(p.tilesN) * p.tilesK;
     const uint32_t steps = std::max(1u, ceilDiv(rows, 64u));
-    const double stepUs = 0.4, tileUs = p.cg * 128.0 * 256 * 4 * 2 / 5e6; // 64 rows; a partial tile out and in
+    const double stepUs = 0.4, tileUs = p.cg * 128.0 * 256 * 4 * 2 / 1e7; // 64 rows; a partial tile out and in
     double best = 0;
     const uint32_t most = uint32_t(std::min(double(steps), std::max(4.0, 2 * kSms / (tiles * p.cg))));
     for (uint32_t splits = 1; splits <= most; ++splits) {
@@ -765,7 +777,12 @@ void launchTiles(const GradArgs& g, const Plan& p, int type, cudaStream_t stream
     config.numAttrs = 1;
     checkCudaCall(cudaLaunchKernelEx(&config, kernel, mapDy, mapQ, mapDw, g));
     if (p.splits > 1) {
-        sumPartials<CG><<<p.tilesN * p.tilesK * CG * (128 * 256 / 4 / 32), 256, 0, stream>>>(g, p.splits);
+        // Few ranges: one thread's loads of a column are in flight together. Many: the columns are few.
+        const uint32_t columns = p.tilesN * p.tilesK * CG * (128 * 256 / 4);
+        if (p.splits <= 8)
+            sumPartials<CG, 1><<<columns / 256, 256, 0, stream>>>(g, p.splits);
+        else
+            sumPartials<CG, 8><<<columns / 32, 256, 0, stream>>>(g, p.splits);
         checkCudaCall(cudaGetLastError());
     }
 }
