@@ -91,14 +91,15 @@ def _shaped(name: str, t, rows: int, cols: int, device: int) -> int:
 def _scales(name: str, t, device: int, rows: int, cols: int, row_blocks: bool = True, square_blocks: bool = True) -> int:
     """Checks the scale bytes of a [rows, cols] matrix and returns the rows per block."""
     wide = (cols + 127) >> 7
-    if not isinstance(t, _torch.Tensor):
+    try:
+        if t.dtype in _SCALES and t.get_device() == device and t.is_contiguous():
+            shape = t.shape
+            if row_blocks and shape == (rows, wide):
+                return 1
+            if square_blocks and shape == ((rows + 127) >> 7, wide):
+                return BLOCK
+    except (AttributeError, TypeError):
         _refuse(f"{name} must be a CUDA tensor")
-    if t.dtype in _SCALES and t.get_device() == device and t.is_contiguous():
-        shape = t.shape
-        if row_blocks and shape == (rows, wide):
-            return 1
-        if square_blocks and shape == ((rows + 127) >> 7, wide):
-            return BLOCK
     if t.dtype not in _SCALES:
         _refuse(f"{name} must hold scale bytes (uint8 or float8_e8m0fnu)")
     if t.get_device() != device:
