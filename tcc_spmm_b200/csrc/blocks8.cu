@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 8 : 6) // warps for
         return;
     const uint32_t left = cols - p.col;
     const bool whole = left >= kBlock;
-    const float scale = scaleValue(scales[p.row * colBlocks + p.col / kBlock]);
+    const float scale = slopeScale(scales[p.row * colBlocks + p.col / kBlock]);
     uint32_t w[kPieces][kE / 4], raw[R::kWords];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)

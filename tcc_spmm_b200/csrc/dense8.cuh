@@ -218,7 +218,12 @@ template <int A> __device__ __forceinline__ void activation(float& x, float& y) 
         x *= logistic(x), y *= logistic(y);
     }
 }
-// f' of two values, in place.
+// The scale of a checkpoint's block for the slopes below: 2^e up to 2^20, NaN for 255. From there on every
+// element but 0 is beyond 2^20 in size, where a slope is exactly 0 or 1 whatever the size; kept to that, x^ stays
+// a float (an element may stand for 2^128) and its square does not overflow (infinity times a factor of 0).
+__device__ __forceinline__ float slopeScale(uint32_t byte) { return scaleValue(byte == 255u ? byte : min(byte, 147u)); }
+
+// f' of two values, in place: NaN, or below 2^60 in size.
 template <int A> __device__ __forceinline__ void activationSlope(float& x, float& y) {
     if constexpr (A == kRelu) {
         x = x > 0.0f ? 1.0f : x == x ? 0.0f : x, y = y > 0.0f ? 1.0f : y == y ? 0.0f : y;

@@ -1,0 +1,62 @@
+"""The dense operators on 8-bit blocks at the ends of the number range, against their definitions in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import tcc_spmm_b200 as T
+from tests import dense8_util as D
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["relu", "silu", "gelu", "gelu_tanh"]
+
+
+def checkpoint(x, kind):
+    y = None if kind == "identity" else torch.empty_like(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device="cuda")
+    scales = torch.empty(x.shape[0], -(-x.shape[1] // 128), dtype=torch.uint8, device="cuda")
+    T.activation_checkpoint_int8(x, y, q, scales, activation=kind)
+    return y, q, scales
+
+
+def large_rows(dtype):
+    """Blocks whose largest element runs up to the type's ends: rows of one value, of its negative, and a row that
+    is masked with the lowest value in places."""
+    top = torch.finfo(dtype).max
+    sizes = [v for v in (1e4, 1e10, 2.0 ** 66, 1e25, 3e38, top) if v <= top]
+    x = torch.zeros(3 * len(sizes), 200, device="cuda")
+    for i, v in enumerate(sizes):
+        x[3 * i] = v
+        x[3 * i + 1] = -v
+        x[3 * i + 2] = torch.linspace(-2, 2, 200, device="cuda")
+        x[3 * i + 2, ::7] = -v
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_functions_of_large_values(dtype, kind):
+    """From 1e4 on every function is x or 0, and its slope 1 or 0; a value that is kept as zero has the slope of
+    zero. An element may stand for 2^128, which no float holds: its slope is still the definition's."""
+    x = large_rows(D.TYPES[dtype])
+    y, q, scales = checkpoint(x, kind)
+    want_q, want_scales = D.quantize(x, "int8")
+    assert torch.equal(scales, want_scales) and torch.equal(q.double(), want_q)
+    far = x.abs() >= 1e4
+    assert torch.equal(y[far], x[far].clamp(min=0))
+    want = D.activation(x.double(), kind)
+    # |x| <= 2 elsewhere: a dozen fp32 roundings and the type's own
+    assert ((y.double() - want).abs()[~far] <= (D.half_step(x.dtype) + 32 * D.U) * want.abs()[~far] + 2.0 ** -24).all()
+    xh = D.values(q, scales)
+    assert (xh[far].abs() >= 9e3).all()  # kept within half a step, a 2^-7th of the block's largest at most
+    for grad in (torch.float32, torch.bfloat16, torch.float16):
+        dy = D.make(*x.shape, grad, 3)
+        dx = torch.empty_like(dy)
+        T.activation_backward_int8(dy, q, scales, dx, activation=kind)
+        assert torch.equal(dx[far], torch.where(xh > 0, dy, torch.zeros_like(dy))[far])
+        zero = xh == 0
+        want = dy.double()[zero] * (0.0 if kind == "relu" else 0.5)
+        least = 2.0 ** -25 if grad == torch.float16 else 2.0 ** -130
+        assert ((dx.double()[zero] - want).abs() <= (D.half_step(grad) + 32 * D.U) * want.abs() + least).all()
+        assert not dx.isnan().any()
