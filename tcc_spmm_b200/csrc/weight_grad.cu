@@ -2,7 +2,8 @@
 //   dW[n, k] (+)= sum over rows r of dy[r, n] * q[r, k] 2^e[r, k / 128]
 //
 // The sum runs on the tensor cores in bf16 with FP32 accumulators, and no operand is rounded: an
-// INT8 element times a power of two has at most 8 significant bits, which bf16 holds, and dy is
+// INT8 element times a power of two has at most 8 significant bits, which bf16 holds (at half its
+// value, since an element may stand for 2^128; what leaves the accumulator is doubled), and dy is
 // split into P bf16 parts that add up to it (P = 1 for bf16, 2 for fp16: 8 + 3 bits, 3 for fp32:
 // 8 + 8 + 8 bits), each multiplied on its own into the same accumulator.
 //
@@ -77,7 +78,7 @@ template <typename T, int CG> struct GradTile {
     static constexpr int kSteps = kP * kRows / 16;      // MMAs per stage
     static constexpr uint32_t kFlush = 60 / kSteps;     // stages between two flushes
     static constexpr int kRawOff = kStages * kBBytes;
-    static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // a raw stage's scales as bf16 pairs, by box and row
+    static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes; // halves of a raw stage's scales as bf16 pairs, by box and row
     static constexpr int kScaleBytes = kRows * kBBoxes * 4;
     static constexpr int kBarOff = kScaleOff + kRaw * kScaleBytes;
     // rawFull, rawEmpty [kRaw]; full, empty, peerFull [kStages]; accFull, accEmpty; TMEM address
@@ -191,9 +192,10 @@ __device__ __forceinline__ void int8ToBf16(uint32_t w, uint32_t scale, uint32_t&
     }
     lo = out[0], hi = out[1];
 }
-// 2^e of a scale byte as a bf16 pair (NaN for 255, a subnormal for 0).
-__device__ __forceinline__ uint32_t scalePair(uint32_t byte) {
-    return (byte == 255u ? 0x7FC0u : byte == 0u ? 0x0040u : byte << 7) * 0x10001u;
+// Half the 2^e of a scale byte as a bf16 pair (NaN for 255, subnormal for 1 and 0). With the whole of it
+// the elements that stand for 2^128 were infinite and made every sum that a zero of dy met them in NaN.
+__device__ __forceinline__ uint32_t halfScalePair(uint32_t byte) {
+    return (byte == 255u ? 0x7FC0u : byte <= 1u ? 0x0020u << byte : (byte - 1u) << 7) * 0x10001u;
 }
 
 // Lane of a 32-lane quarter of A and D -> column of dy within the quarter's 32: the 16-lane store
@@ -285,7 +287,7 @@ __device__ __forceinline__ void loadRaw(const GradArgs& p, uint32_t base, uint32
 #pragma unroll
         for (int box = 0; box < L::kBBoxes; ++box)
             if (scaleRow < uint32_t(L::kRows))
-                stsU32(scales + 4 * (box * L::kRows + scaleRow), scalePair(scale[box]));
+                stsU32(scales + 4 * (box * L::kRows + scaleRow), halfScalePair(scale[box]));
         dev::cpAsyncArriveNoinc(rawFull + 8 * raw);
         if (++raw == L::kRaw)
             raw = 0, phase ^= 1;
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                 dev::tcWaitLd();
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    sum[c + i] += __uint_as_float(r[i]);
+                    sum[c + i] = fmaf(__uint_as_float(r[i]), 2.0f, sum[c + i]); // B holds half of q^
             }
             dev::tcFenceBefore();
             __syncwarp();
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
                             ok = waitPhase(rawEmpty + 8 * raw, (stage / L::kRaw + 1) & 1);
 #pragma unroll
                             for (int i = 0; i < kLoads; ++i)
-                                stsU32(base + L::kScaleOff + raw * L::kScaleBytes + 4 * (32 * i + lane), scalePair(held[u][i]));
+                                stsU32(base + L::kScaleOff + raw * L::kScaleBytes + 4 * (32 * i + lane), halfScalePair(held[u][i]));
                             __syncwarp();
                             if (lane == 0)
                                 dev::mbarArrive(rawFull + 8 * raw);

@@ -60,3 +60,47 @@ def test_functions_of_large_values(dtype, kind):
         least = 2.0 ** -25 if grad == torch.float16 else 2.0 ** -130
         assert ((dx.double()[zero] - want).abs() <= (D.half_step(grad) + 32 * D.U) * want.abs() + least).all()
         assert not dx.isnan().any()
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("n", [8, 200])  # one CTA a tile of dW, or two
+@pytest.mark.parametrize("grad", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_weight_grad_of_large_values(dtype, grad, n, aligned):
+    """Large elements meet zeros of dy (sums that leave them out) and, one to a sum, small values of dy, with which
+    even 2^128 gives a finite product. A sum of one product is exact in fp32 (8 bits of x^ by up to 11 of dy)."""
+    x = large_rows(D.TYPES[dtype])
+    _, q, scales = checkpoint(x, "identity")
+    rows, k = x.shape
+    dy = torch.zeros(rows, n)
+    for j in range(n):
+        if j < rows:
+            dy[j, j] = 0.75 * 2.0 ** -8 * (-1) ** j
+    off = 0 if aligned else 1
+    held = D.strided(rows, n, D.TYPES[grad], D.up16(n) + off, off)
+    held.copy_(dy)
+    kept = D.strided(rows, k, torch.int8, D.up16(k) + off, off)
+    kept.copy_(q)
+    dw = torch.full((n, k), float("nan"), device="cuda")
+    T.weight_grad_int8(held, kept, scales, dw)
+    xh = D.values(q, scales)
+    want = dy.cuda().double().t() @ xh
+    assert xh.abs().max() == 2.0 ** 128 and torch.equal(dw.double(), want)
+    T.weight_grad_int8(held, kept, scales, dw, accumulate=True)
+    assert torch.equal(dw.double(), 2 * want)
+
+
+@pytest.mark.parametrize("grad", ["fp32", "bf16"])
+@pytest.mark.parametrize("byte", [0, 1, 2, 3])
+def test_weight_grad_of_the_smallest_scales(byte, grad):
+    """The scales at the lower end (0 is the format's, the quantizers write no less than 1) with a dy that brings
+    the sums back into range: every product is exact."""
+    rows, n, k = 70, 20, 255
+    q = (torch.arange(rows * k).reshape(rows, k) % 255 - 127).to(torch.int8).cuda()
+    scales = torch.full((rows, 2), byte, dtype=torch.uint8, device="cuda")
+    dy = torch.zeros(rows, n, device="cuda")
+    dy[:, 0], dy[3, 1], dy[69, 19] = 2.0 ** 60, -2.0 ** 100, 2.0 ** 126
+    dw = torch.empty(n, k, device="cuda")
+    T.weight_grad_int8(dy.to(D.TYPES[grad]), q, scales, dw)
+    want = dy.double().t() @ D.values(q, scales)
+    assert torch.equal(dw.double(), want)
