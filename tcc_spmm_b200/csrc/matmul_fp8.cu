@@ -99,13 +99,27 @@ template <typename T> void launchGeneric(const Product& p) {
     checkCudaCall(cudaGetLastError());
 }
 
+// A scale 2^e (NaN for the byte 255) as two factors of about half its exponent, the larger first. The product
+// of two scales may be beyond the floats where a sum times it is none (zero times infinity) or is one; so a sum
+// is multiplied by a.large * b.small and then by a.small * b.large, which are floats for all bytes and both
+// on one side of 1.
+struct Halves {
+    float large, small;
+};
+__device__ __forceinline__ Halves halves(uint32_t byte) { // exponents byte - byte / 2 - 63 and byte / 2 - 64
+    return {__uint_as_float(byte == 255u ? 0x7FC00000u : (byte - byte / 2 + 64u) << 23), __uint_as_float((byte / 2 + 63u) << 23)};
+}
+__device__ __forceinline__ float timesScales(float sum, Halves a, Halves b) {
+    return sum * (a.large * b.small) * (a.small * b.large);
+}
+
 // ---- few rows of a ------------------------------------------------------------------------------
 // With up to 16 rows of a the product is a read of b. A CTA takes 16 rows of b; its warps take blocks of
 // 128 of k in turn, each with a ring of its own of asynchronous copies (no barrier between warps, and
 // all of a 4096-wide row in flight at once), and their sums are added up in shared memory at the end, in
 // a fixed order. The order of k in mma.m16n8k32 may be any that both operands share, so a lane reads 16
 // bytes of k of two rows of b and of MT rows of a at a time: two MMAs per 64 of k and 8 rows of a. The sum
-// over a block is multiplied by the two scales' product, a power of two. 7.2 us for 1 x 4096 x 4096 out of
+// over a block is multiplied by the two scales, powers of two (see Halves). 7.2 us for 1 x 4096 x 4096 out of
 // HBM (2.3 TB/s; 2.4 us of it launch and drain), 20.9 us for 1 x 8192 x 8192 (3.2 TB/s).
 template <int MT_> struct Few {
     static constexpr int MT = MT_;
@@ -198,15 +212,14 @@ __global__ void __launch_bounds__(32 * Few<MT>::kWarps)
                 mmaFp8<B5, A5>(part[j], u.z, v.z, u.w, v.w, x.z, x.w);
             }
         }
-        const float sb[2] = {scaleValue(scales[g * kBlocks + kb]), scaleValue(scales[(g + 8) * kBlocks + kb])};
+        const Halves sb[2] = {halves(scales[g * kBlocks + kb]), halves(scales[(g + 8) * kBlocks + kb])};
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             const unsigned char* sa = scales + (L::kRows + 8 * j + 2 * t) * kBlocks + kb;
-            const float s0 = scaleValue(sa[0]), s1 = scaleValue(sa[kBlocks]);
-            acc[j][0] = fmaf(part[j][0], sb[0] * s0, acc[j][0]);
-            acc[j][1] = fmaf(part[j][1], sb[0] * s1, acc[j][1]);
-            acc[j][2] = fmaf(part[j][2], sb[1] * s0, acc[j][2]);
-            acc[j][3] = fmaf(part[j][3], sb[1] * s1, acc[j][3]);
+            const Halves s[2] = {halves(sa[0]), halves(sa[kBlocks])};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[j][i] += timesScales(part[j][i], s[i % 2], sb[i / 2]);
         }
         __syncwarp(); // every lane has read the stage
         if (kb + L::kStages * L::kWarps < kBlocks)

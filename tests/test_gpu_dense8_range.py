@@ -104,3 +104,67 @@ def test_weight_grad_of_the_smallest_scales(byte, grad):
     T.weight_grad_int8(dy.to(D.TYPES[grad]), q, scales, dw)
     want = dy.double().t() @ D.values(q, scales)
     assert torch.equal(dw.double(), want)
+
+
+# ---- product --------------------------------------------------------------------------------------
+# The kernels of the product: up to 8 and up to 16 rows, tiles, tiles that share k, and [k, n] weights.
+FORMS = [(3, 40, 300, "nk", True), (13, 40, 300, "nk", True), (130, 140, 300, "nk", True), (140, 150, 1100, "nk", True),
+         (130, 140, 300, "kn", True), (130, 140, 1100, "kn", True)]
+
+
+def blocks(rows, cols, kind, aligned, q64):
+    held = D.strided(rows, cols, D.FP8[kind], D.up16(cols) if aligned else cols + 1, 0 if aligned else 1)
+    held.view(torch.uint8).copy_(q64.float().to(D.FP8[kind]).view(torch.uint8))
+    return held
+
+
+def small_elements(rows, cols, seed):
+    """Whole numbers from -2 to 2."""
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randint(-2, 3, (rows, cols), generator=gen).double().cuda()
+
+
+@pytest.mark.parametrize("m,n,k,layout,aligned", FORMS)
+def test_product_of_extreme_scales(m, n, k, layout, aligned):
+    """Scales whose product no float holds, in either direction, beside sums that are zero or bring it back. Every
+    sum is a small whole number times a power of two: exact in fp32."""
+    qa, qb = small_elements(m, k, 1), small_elements(n, k, 2)
+    kb, nb = -(-k // 128), -(-n // 128)
+    for kind, factor, a_byte, b_byte in (("e4m3", 0, 254, 254), ("e4m3", 1, 1, 1), ("e5m2", 28672, 52, 52), ("e4m3", 224, 1, 254),
+                                         ("e4m3", 224, 254, 1), ("e4m3", 224, 200, 60), ("e4m3", 1, 0, 254)):
+        a64, b64 = qa * max(factor, 1), qb * max(factor, 1)
+        if factor == 0:  # 2^254: only zeros may meet
+            a64[:, ::2] = 0
+            b64[:, 1::2] = 0
+        a = blocks(m, k, kind, aligned, a64)
+        b = blocks(n, k, kind, aligned, b64) if layout == "nk" else blocks(k, n, kind, aligned, b64.t())
+        sa = torch.full((m, kb), a_byte, dtype=torch.uint8, device="cuda")
+        sb = torch.full((nb, kb) if layout == "nk" else (kb, nb), b_byte, dtype=torch.uint8, device="cuda")
+        y = torch.full((m, n), float("nan"), device="cuda")
+        T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
+        want = (a64 @ b64.t()) * 2.0 ** (a_byte + b_byte - 254)
+        assert torch.equal(y, want.float()), (kind, a_byte, b_byte)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("m,n,k,layout,aligned", FORMS)
+def test_product_of_large_values(m, n, k, layout, aligned, kind):
+    """The largest finite rows, whose elements stand for 2^128: zeros of b leave them out, and a small b brings them
+    into range."""
+    x = torch.zeros(m, k, device="cuda")
+    x[0::3] = torch.finfo(torch.float32).max
+    x[1::3, ::5] = torch.finfo(torch.float32).min
+    sa = torch.empty(m, -(-k // 128), dtype=torch.uint8, device="cuda")
+    a = blocks(m, k, kind, aligned, torch.zeros(m, k))
+    T.quantize_blocks_fp8(x, a, sa)
+    want_q, want_s = D.quantize(x, kind)
+    assert torch.equal(a.double(), want_q) and torch.equal(sa, want_s)
+    b64 = torch.zeros(n, k, device="cuda", dtype=torch.float64)
+    b64[::2, 35], b64[1::4, 260] = 1.0, -0.5
+    nb, kb = -(-n // 128), -(-k // 128)
+    b = blocks(n, k, "e4m3", aligned, b64) if layout == "nk" else blocks(k, n, "e4m3", aligned, b64.t())
+    sb = torch.full((nb, kb) if layout == "nk" else (kb, nb), 127 - 20, dtype=torch.uint8, device="cuda")
+    y = torch.full((m, n), float("nan"), device="cuda")
+    T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
+    want = D.values(a, sa) @ b64.t() * 2.0 ** -20
+    assert torch.equal(y.double(), want) and want.abs().max() == 2.0 ** 108
