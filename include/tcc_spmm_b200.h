@@ -305,7 +305,9 @@ int tcc_spmm_launch_shape(uint32_t features, int variant, uint32_t* grid, uint32
  * INT8; e >= -126; 2^0 for a block of zeros), and its elements are x * 2^-e rounded to nearest,
  * ties to even. scales[row block][column block] holds e + 127 as a byte (E8M0), contiguous,
  * ceil(cols / 128) bytes per row of blocks. A block that holds an infinity or NaN has the scale
- * byte 255 (NaN) and elements NaN (INT8: 0), and all that is computed from it is NaN.
+ * byte 255 (NaN) and elements NaN (INT8: 0), and all that is computed from it is NaN. Where absmax is
+ * above 127 * 2^121 (INT8; 240 * 2^120, 28672 * 2^113) its element may round to 2^128, which fp32 does
+ * not hold; the operators below compute with that value and give infinity only where a result is one.
  *
  * Strides are row strides in elements, at least the row's width; elements of a row are adjacent.
  * Sizes from 0 to 2^32 - 256 are allowed. The matrices of a call must not overlap, but for y == x

@@ -31,43 +31,62 @@ __device__ __forceinline__ float fp8Value(uint8_t v, bool e4m3) {
     return __half2float(__half(h));
 }
 
+// A scale 2^e (NaN for the byte 255) as two factors of about half its exponent, the larger first. The product
+// of two scales may be beyond the floats where a sum times it is none (zero times infinity) or is one; so a sum
+// is multiplied by a.large * b.small and then by a.small * b.large, which are floats for all bytes and both
+// on one side of 1.
+struct Halves {
+    float large, small;
+};
+__device__ __forceinline__ Halves halves(uint32_t byte) { // exponents byte - byte / 2 - 63 and byte / 2 - 64
+    return {__uint_as_float(byte == 255u ? 0x7FC00000u : (byte - byte / 2 + 64u) << 23), __uint_as_float((byte / 2 + 63u) << 23)};
+}
+__device__ __forceinline__ float timesScales(float sum, Halves a, Halves b) {
+    return sum * (a.large * b.small) * (a.small * b.large);
+}
+
 // ---- any strides and alignment ----------------------------------------------------------------
-// 64 x 64 outputs per CTA, 4 x 4 per thread, FP32 FMA from operands dequantized into shared memory.
+// 64 x 64 outputs per CTA, 4 x 4 per thread, FP32 FMA from elements widened into shared memory; the sum over a
+// block of 128 is multiplied by its two scales.
 // For matrices whose rows do not start on 16 bytes, which the tensor-core kernels' copies cannot read.
-// FMA and shared-memory bound: 21 TFLOP/s at 8192 x 4096 x 4096.
+// FMA and shared-memory bound: 12.2 ms for 8192 x 4096 x 4100 on rows of 4101 bytes, 22.6 TFLOP/s.
 constexpr int kTile = 64, kStep = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(256) productGeneric(const Operand a, const Operand b, bool kn, const float* __restrict__ bias,
                                                       T* __restrict__ out, uint64_t outStride, uint32_t m, uint32_t n,
                                                       uint32_t k, uint32_t tilesN) {
+    static_assert(kBlock % kStep == 0, "a step lies in one block");
     __shared__ float as[kStep][kTile + 1], bs[kStep][kTile + 1];
+    __shared__ Halves aScale[kTile], bScale[kTile];
     const uint32_t m0 = blockIdx.x / tilesN * kTile, n0 = blockIdx.x % tilesN * kTile;
     const uint32_t kBlocks = (k + kBlock - 1) / kBlock, nBlocks = (n + kBlock - 1) / kBlock;
     const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {};
+    float acc[4][4] = {}, part[4][4] = {};
     for (uint32_t k0 = 0; k0 < k; k0 += kStep) {
+        const uint32_t block = k0 / kBlock;
+        if (k0 % kBlock == 0 && threadIdx.x < 2 * kTile) { // rows and columns outside: their sums go nowhere
+            const uint32_t i = threadIdx.x % kTile, row = min(m0 + i, m - 1), col = min(n0 + i, n - 1);
+            if (threadIdx.x < kTile)
+                aScale[i] = halves(a.scales[uint64_t(row >> a.rowShift) * kBlocks + block]);
+            else
+                bScale[i] = halves(kn ? b.scales[uint64_t(block) * nBlocks + col / kBlock]
+                                      : b.scales[uint64_t(col >> b.rowShift) * kBlocks + block]);
+        }
         for (uint32_t i = threadIdx.x; i < kStep * kTile; i += 256) {
             {
                 const uint32_t kk = i % kStep, r = i / kStep;
                 const uint32_t row = m0 + r, col = k0 + kk;
                 float v = 0.0f;
                 if (row < m && col < k)
-                    v = fp8Value(a.data[row * a.stride + col], a.type == TCC_E4M3) *
-                        scaleValue(a.scales[uint64_t(row >> a.rowShift) * kBlocks + col / kBlock]);
+                    v = fp8Value(a.data[row * a.stride + col], a.type == TCC_E4M3);
                 as[kk][r] = v;
             }
             const uint32_t kk = kn ? i / kTile : i % kStep, r = kn ? i % kTile : i / kStep;
             const uint32_t row = n0 + r, col = k0 + kk;
             float v = 0.0f;
-            if (row < n && col < k) {
-                if (kn)
-                    v = fp8Value(b.data[col * b.stride + row], b.type == TCC_E4M3) *
-                        scaleValue(b.scales[uint64_t(col >> b.rowShift) * nBlocks + row / kBlock]);
-                else
-                    v = fp8Value(b.data[row * b.stride + col], b.type == TCC_E4M3) *
-                        scaleValue(b.scales[uint64_t(row >> b.rowShift) * kBlocks + col / kBlock]);
-            }
+            if (row < n && col < k)
+                v = fp8Value(kn ? b.data[col * b.stride + row] : b.data[row * b.stride + col], b.type == TCC_E4M3);
             bs[kk][r] = v;
         }
         __syncthreads();
@@ -77,7 +96,15 @@ __global__ void __launch_bounds__(256) productGeneric(const Operand a, const Ope
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx + 16 * j], acc[i][j]);
+                    part[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx + 16 * j], part[i][j]);
+        if (k0 % kBlock == kBlock - kStep || k - k0 <= kStep)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[i][j] += timesScales(part[i][j], aScale[ty * 4 + i], bScale[tx + 16 * j]);
+                    part[i][j] = 0.0f;
+                }
         __syncthreads();
     }
 #pragma unroll
@@ -97,20 +124,6 @@ template <typename T> void launchGeneric(const Product& p) {
     productGeneric<T><<<uint32_t(grid), 256, 0, p.stream>>>(p.a, p.b, p.kn, p.bias, static_cast<T*>(p.out), p.outStride,
                                                             p.m, p.n, p.k, tilesN);
     checkCudaCall(cudaGetLastError());
-}
-
-// A scale 2^e (NaN for the byte 255) as two factors of about half its exponent, the larger first. The product
-// of two scales may be beyond the floats where a sum times it is none (zero times infinity) or is one; so a sum
-// is multiplied by a.large * b.small and then by a.small * b.large, which are floats for all bytes and both
-// on one side of 1.
-struct Halves {
-    float large, small;
-};
-__device__ __forceinline__ Halves halves(uint32_t byte) { // exponents byte - byte / 2 - 63 and byte / 2 - 64
-    return {__uint_as_float(byte == 255u ? 0x7FC00000u : (byte - byte / 2 + 64u) << 23), __uint_as_float((byte / 2 + 63u) << 23)};
-}
-__device__ __forceinline__ float timesScales(float sum, Halves a, Halves b) {
-    return sum * (a.large * b.small) * (a.small * b.large);
 }
 
 // ---- few rows of a ------------------------------------------------------------------------------

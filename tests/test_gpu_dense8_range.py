@@ -107,9 +107,10 @@ def test_weight_grad_of_the_smallest_scales(byte, grad):
 
 
 # ---- product --------------------------------------------------------------------------------------
-# The kernels of the product: up to 8 and up to 16 rows, tiles, tiles that share k, and [k, n] weights.
+# Every kernel of the product: up to 8 and up to 16 rows, tiles, tiles that share k, [k, n] weights, and operands
+# whose rows are off 16 bytes.
 FORMS = [(3, 40, 300, "nk", True), (13, 40, 300, "nk", True), (130, 140, 300, "nk", True), (140, 150, 1100, "nk", True),
-         (130, 140, 300, "kn", True), (130, 140, 1100, "kn", True)]
+         (130, 140, 300, "kn", True), (130, 140, 1100, "kn", True), (3, 140, 300, "nk", False), (130, 70, 300, "kn", False)]
 
 
 def blocks(rows, cols, kind, aligned, q64):
