@@ -250,7 +250,9 @@ __device__ __forceinline__ void copyRow(const uint8_t* src, const void* valid, i
     }
 }
 // One of the three warps that fill raw stages without TMA: rows warp, warp + 3, ..., pieces of WA bytes
-// of dy and WB bytes of q. Every lane arrives on the stage's barrier once its copies have landed.
+// of dy and WB bytes of q. Every lane arrives on the stage's barrier once its asynchronous copies have landed; that
+// arrival does not publish the lane's ordinary stores (scales, pieces of 2 and 1 bytes), so a warp arrives once
+// more, after them.
 template <typename T, int CG, int WA, int WB>
 __device__ __forceinline__ void loadRaw(const GradArgs& p, uint32_t base, uint32_t rawFull, uint32_t rawEmpty, uint32_t warp,
                                         uint32_t lane, uint64_t begin, uint64_t end, uint32_t stages, uint32_t n0,
@@ -289,6 +291,9 @@ __device__ __forceinline__ void loadRaw(const GradArgs& p, uint32_t base, uint32
             if (scaleRow < uint32_t(L::kRows))
                 stsU32(scales + 4 * (box * L::kRows + scaleRow), halfScalePair(scale[box]));
         dev::cpAsyncArriveNoinc(rawFull + 8 * raw);
+        __syncwarp();
+        if (lane == 0)
+            dev::mbarArrive(rawFull + 8 * raw);
         if (++raw == L::kRaw)
             raw = 0, phase ^= 1;
     }
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(GradTile<T, CG>::kThreads, 1)
     const uint32_t rank = CG == 1 ? 0 : clusterRank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kRaw; ++i)
-            dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 96), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
+            dev::mbarInit(rawFull + 8 * i, TMA ? 2 : 3 * (32 + 1)), dev::mbarInit(rawEmpty + 8 * i, 8); // 4 warps of A, 4 of B
         for (int i = 0; i < L::kStages; ++i)
             dev::mbarInit(full + 8 * i, 8), dev::mbarInit(empty + 8 * i, 1), dev::mbarInit(peerFull + 8 * i, 1);
         dev::mbarInit(accFull, 1), dev::mbarInit(accEmpty, 8 * CG);
