@@ -289,9 +289,10 @@ template <int MT> void launchFew(const Product& p) {
 // E8M0 scales are the blocks' own bytes: the hardware takes one scale per 32 elements of k, and a
 // block's four groups take the same one, so no scale is applied outside the tensor core and the sum
 // over k stays in one FP32 accumulator in tensor memory. The tensor core cuts off what an addition
-// shifts out below the accumulator's last bit, about 1e-8 of the sum for every MMA (measured; 1.4e-6
-// after 128), so where the output shows it (fp32) the accumulator is emptied into registers, which
-// round to nearest, every kPass blocks. Scales travel as words of four
+// shifts out below the accumulator's last bit: measured, 1.4e-6 of the sum of absolute values after 128 MMAs on
+// operands of either sign, and 2.4e-3 after 32768 (7e-8 for every MMA) where all terms have one sign. So a long sum
+// is emptied into registers, which round to nearest, every kPass blocks (mostBlocks says which sums are long); that
+// also bounds how long the epilogue waits. Scales travel as words of four
 // consecutive blocks per row, loaded by warps of their own, copied to tensor memory by the MMA thread
 // and picked by the byte selector of the instruction descriptor. Eight warps bring finished tiles into
 // registers, release the accumulator, and write them by TMA through 4 KB of shared memory each.
@@ -519,7 +520,7 @@ __device__ __forceinline__ void storeEight(const ProductArgs& p, uint64_t row, u
     }
 }
 
-// LONG: fp32 output of a k of more than kPass blocks, whose accumulators are summed in registers.
+// LONG: more blocks of k than mostBlocks, whose accumulators are summed in registers.
 // SPLIT: few tiles: the cluster's CTAs (p.splitBlocks blocks of k each) share one tile; each leaves its
 // sums in its shared memory and adds up an equal part of the columns of all of them, in the order of k.
 template <int BN, int CG, bool KN, bool LONG, bool SPLIT>
@@ -794,9 +795,9 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
                             for (int j = 0; j < 8; ++j)
                                 v[j] += ldClusterF32(mine + 128 * (c + j), s);
                         if (row0 + lane < p.m && n0 + c < p.n) {
-                            if (!LONG && p.outType == TCC_BF16)
+                            if (p.outType == TCC_BF16)
                                 storeEight<__nv_bfloat16>(p, row0 + lane, n0 + c, v, bias + 4 * c);
-                            else if (LONG || p.outType == TCC_F32)
+                            else if (p.outType == TCC_F32)
                                 storeEight<float>(p, row0 + lane, n0 + c, v, bias + 4 * c);
                             else
                                 storeEight<__half>(p, row0 + lane, n0 + c, v, bias + 4 * c);
@@ -807,9 +808,9 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
             if (!ok)
                 break;
             if (row0 < p.m && n0 < p.n) {
-                if (!LONG && p.outType == TCC_BF16)
+                if (p.outType == TCC_BF16)
                     storeTile<L, __nv_bfloat16>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
-                else if (LONG || p.outType == TCC_F32)
+                else if (p.outType == TCC_F32)
                     storeTile<L, float>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
                 else
                     storeTile<L, __half>(p, &mapOut, r, buf, turn, bias, row0, n0, lane);
@@ -835,6 +836,13 @@ ScaleView scaleView(const Operand& o, uint32_t rows, uint32_t width) {
 
 // Blocks of k of each of a split tile's CTAs: a multiple of 4, as their scales come.
 uint32_t blocksPerSplit(uint32_t kBlocks, uint32_t splits) { return ceilDiv(ceilDiv(kBlocks, splits), 4u) * 4; }
+
+// The most blocks of k that one accumulator sums: kPass for fp32 outputs, and so many for the 16-bit types that the
+// loss of 7e-8 for each of a block's four MMAs stays below a tenth of a half step (fp16 3.7e-5 of 4.9e-4, bf16
+// 2.9e-4 of 3.9e-3). Emptying it takes 8192 x 4096 x 16512 from 385 us (bf16, one accumulator) to 407 (fp16).
+template <typename L> constexpr uint32_t mostBlocks(int outType) {
+    return outType == TCC_F32 ? L::kPass : outType == TCC_F16 ? 128u : 1024u;
+}
 
 template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Product& p, uint32_t splits = 1) {
     using L = Tile<BN, CG>;
@@ -889,7 +897,7 @@ template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Pr
     attr.val.clusterDim.x = SPLIT ? splits : CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    if (p.outType == TCC_F32 && (SPLIT ? args.splitBlocks : kBlocks) > L::kPass) {
+    if ((SPLIT ? args.splitBlocks : kBlocks) > mostBlocks<L>(p.outType)) {
         allowSharedMemory<productTiles<BN, CG, KN, true, SPLIT>>(L::kBytes);
         checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN, true, SPLIT>, mapA, mapB, mapOut, args));
     } else {
