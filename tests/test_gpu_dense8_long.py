@@ -47,3 +47,48 @@ def test_product_long_sums(m, n, k, layout):
         off = ((y.double() - want).abs() / want).max()
         assert off <= limit, (dtype, float(off), limit)
     assert T.device_status() == 0
+
+
+def test_product_long_sums_shared_by_ctas():
+    """fp32 outputs of few tiles of [n, k] weights: CTAs that share k and empty their accumulators on the way."""
+    m, n, k = 600, 900, 8192
+    a, b = positive(m, k, 0.5, 2.0, 3), positive(n, k, 0.01, 0.12, 4)
+    sa = torch.randint(125, 130, (m, k // 128), generator=torch.Generator().manual_seed(5)).to(torch.uint8).cuda()
+    sb = torch.randint(125, 130, (8, k // 128), generator=torch.Generator().manual_seed(6)).to(torch.uint8).cuda()
+    want = D.values(a, sa) @ D.values(b, sb, 128).t()
+    for dtype, kept in ((torch.float32, 64), (torch.bfloat16, 256), (torch.float16, 256)):
+        y = torch.full((m, n), float("nan"), device="cuda", dtype=dtype)
+        T.matmul_fp8_blocks(a, sa, b, sb, y)
+        # sums of up to four passes, then of up to eight CTAs
+        assert ((y.double() - want).abs() <= (D.half_step(dtype) + kept * D.U + 12 * 2.0 ** -24) * want).all(), dtype
+    assert T.device_status() == 0
+
+
+# one CTA a tile of dW and two: so many tiles that each range of rows is all of them; and so few that ranges are many
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,n,k,ranges", [(6000, 100, 148 * 256, 1), (6001, 512, 37 * 256, 1), (1000000, 30, 70, 100)])
+def test_weight_grad_long_sums(rows, n, k, ranges, dtype, pad):
+    """A range of rows whose accumulator is emptied several times (every 60 MMAs of 16 rows, of which bf16 takes one,
+    fp16 two and fp32 three; 56 at least, since stages are whole), the ranges' sums added in eight sums and those in
+    order."""
+    dt, parts = D.TYPES[dtype], {"bf16": 1, "fp16": 2, "fp32": 3}[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    q = D.strided(rows, k, torch.int8, D.up16(k) + pad, pad)
+    q.copy_(torch.randint(1, 128, (rows, k), device="cuda", generator=gen, dtype=torch.int8))
+    scales = torch.full((rows, -(-k // 128)), 127 - 7, dtype=torch.uint8, device="cuda")
+    dy = D.strided(rows, n, dt, D.up16(n) + pad, pad)
+    dy.copy_(torch.rand(rows, n, device="cuda", generator=gen) * 1.5 + 0.5)
+    cg, size = 1 if n <= 128 else 2, T.weight_grad_int8_workspace_size(rows, n, k)
+    splits = max(1, size // (-(-n // (128 * cg)) * -(-k // 256) * cg * 128 * 256 * 4))
+    assert splits == 1 if ranges == 1 else splits >= ranges
+    flushes = -(-(-(-rows // splits) + 64) * parts // (16 * 56))
+    assert flushes >= 6 * parts
+    dw = torch.full((n, k), float("nan"), device="cuda")
+    T.weight_grad_int8(dy, q, scales, dw)
+    want = dy.double().t() @ q.double() * 2.0 ** -7
+    added = splits if splits <= 8 else -(-splits // 8) + 8
+    limit = 60 * D.U + (flushes + added) * 2.0 ** -24
+    off = ((dw.double() - want).abs() / want).max()
+    assert off <= limit, (float(off), limit)
+    assert T.device_status() == 0
