@@ -150,6 +150,7 @@ TEST_SIGNATURES = {
                                                     C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p,
                                                     C.c_uint32, C.c_int, C.c_void_p]),
     "tcc_test_static_counters_nonzero": (C.c_int, [u64p]),
+    "tcc_test_product_parts": (C.c_uint32, [C.c_uint64, C.c_uint32, u32p, u32p]),
 }
 
 WL_SIGNATURES = {

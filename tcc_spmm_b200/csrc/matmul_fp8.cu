@@ -3,6 +3,8 @@
 #include "dense8.cuh"
 #include "dense8_tc.cuh"
 
+#include <mutex>
+
 namespace tcc {
 namespace {
 
@@ -357,7 +359,7 @@ struct ProductArgs {
     bool keepB; // one column of tiles, and a stage always holds the same block of k: its b stays
     uint32_t m, n, k, tilesM, tilesN;
     uint32_t idesc;
-    uint32_t splits, splitBlocks; // of SPLIT: CTAs per tile (2, 4 or 8), blocks of k each (a multiple of 4)
+    uint32_t splits; // of SPLIT: CTAs per tile (2, 4 or 8)
 };
 
 // Scale bytes of blocks 4g .. 4g + 3 of one row; 1.0 for rows and blocks outside.
@@ -520,8 +522,14 @@ __device__ __forceinline__ void storeEight(const ProductArgs& p, uint64_t row, u
     }
 }
 
+// The first block of k of one of the CTAs that share a tile: groups of four blocks, as their scales come, dealt out
+// evenly.
+__host__ __device__ constexpr uint32_t firstBlock(uint32_t kBlocks, uint32_t part, uint32_t parts) {
+    return (kBlocks + 3) / 4 * part / parts * 4;
+}
+
 // LONG: more blocks of k than mostBlocks, whose accumulators are summed in registers.
-// SPLIT: few tiles: the cluster's CTAs (p.splitBlocks blocks of k each) share one tile; each leaves its
+// SPLIT: few tiles: the cluster's CTAs share one tile's blocks of k (see firstBlock); each leaves its
 // sums in its shared memory and adds up an equal part of the columns of all of them, in the order of k.
 template <int BN, int CG, bool KN, bool LONG, bool SPLIT>
 __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
@@ -557,7 +565,8 @@ __global__ void __launch_bounds__(Tile<BN, CG>::kThreads, 1)
     static_assert(!SPLIT || CG == 1, "a split tile belongs to single CTAs");
     const uint32_t kBlocks = (p.k + kBlock - 1) / kBlock;
     const uint32_t part = SPLIT ? clusterRank() : 0, parts = SPLIT ? p.splits : 1;
-    const uint32_t kbFirst = SPLIT ? part * p.splitBlocks : 0, kbLast = SPLIT ? min(kbFirst + p.splitBlocks, kBlocks) : kBlocks;
+    const uint32_t kbFirst = SPLIT ? firstBlock(kBlocks, part, parts) : 0;
+    const uint32_t kbLast = SPLIT ? min(firstBlock(kBlocks, part + 1, parts), kBlocks) : kBlocks;
     const uint32_t groups = (kbLast - kbFirst + 3) / 4; // kbFirst is a multiple of 4
     const uint32_t tiles = p.tilesM * p.tilesN, firstTile = blockIdx.x / (SPLIT ? parts : CG),
                    tileStep = gridDim.x / (SPLIT ? parts : CG);
@@ -834,9 +843,16 @@ ScaleView scaleView(const Operand& o, uint32_t rows, uint32_t width) {
     return {o.scales, rows, o.rowShift, width, width % 4 == 0 && alignedTo(o.scales, 4)};
 }
 
-// Blocks of k of each of a split tile's CTAs: a multiple of 4, as their scales come.
-uint32_t blocksPerSplit(uint32_t kBlocks, uint32_t splits) { return ceilDiv(ceilDiv(kBlocks, splits), 4u) * 4; }
-
+// How many CTAs share k where there are `tiles` tiles of 128 x 128: one to eight, as long as all the tiles' clusters
+// run at once and each CTA has four blocks of k. clusters: how many of 2, 4 and 8 CTAs run at once, which is less
+// than the SMs would hold since a cluster stays within a GPC (33 of 4 and 15 of 8 on a B200; 16 tiles at k = 8192
+// take 18.6 us with eight CTAs each and 10.9 with four, 14 tiles 10.3 and 10.9).
+constexpr uint32_t ctasPerTile(uint64_t tiles, uint32_t kBlocks, const uint32_t (&clusters)[3]) {
+    uint32_t parts = 1;
+    for (int i = 0; i < 3 && tiles <= clusters[i] && kBlocks >= 8 * parts; ++i)
+        parts *= 2;
+    return parts;
+}
 // The most blocks of k that one accumulator sums: kPass for fp32 outputs, and so many for the 16-bit types that the
 // loss of 7e-8 for each of a block's four MMAs stays below a tenth of a half step (fp16 3.7e-5 of 4.9e-4, bf16
 // 2.9e-4 of 3.9e-3). Emptying it takes 8192 x 4096 x 16512 from 385 us (bf16, one accumulator) to 407 (fp16).
@@ -885,7 +901,6 @@ template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Pr
                              width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
     }
     args.splits = splits;
-    args.splitBlocks = blocksPerSplit(kBlocks, splits);
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(SPLIT ? args.tilesM * args.tilesN * splits
                                 : CG * std::min<uint32_t>(args.tilesM * args.tilesN, multiprocessors() / CG));
@@ -897,13 +912,49 @@ template <int BN, int CG, bool KN, bool SPLIT = false> void launchTiles(const Pr
     attr.val.clusterDim.x = SPLIT ? splits : CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    if ((SPLIT ? args.splitBlocks : kBlocks) > mostBlocks<L>(p.outType)) {
+    if ((SPLIT ? ceilDiv(ceilDiv(kBlocks, 4u), splits) * 4 : kBlocks) > mostBlocks<L>(p.outType)) {
         allowSharedMemory<productTiles<BN, CG, KN, true, SPLIT>>(L::kBytes);
         checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN, true, SPLIT>, mapA, mapB, mapOut, args));
     } else {
         allowSharedMemory<productTiles<BN, CG, KN, false, SPLIT>>(L::kBytes);
         checkCudaCall(cudaLaunchKernelEx(&config, productTiles<BN, CG, KN, false, SPLIT>, mapA, mapB, mapOut, args));
     }
+}
+
+// The clusters of 2, 4 and 8 CTAs that share a tile which run at once on the current device (asked once per device).
+struct SharingClusters {
+    std::atomic<bool> known;
+    uint32_t count[3];
+};
+const uint32_t (&sharingClusters())[3] {
+    static SharingClusters devices[64] = {};
+    static std::mutex asking;
+    static constexpr uint32_t none[3] = {};
+    const int device = currentDevice();
+    if (device >= 64)
+        return none;
+    SharingClusters& d = devices[device];
+    if (!d.known.load(std::memory_order_acquire)) {
+        using L = Tile<128, 1>;
+        const std::lock_guard<std::mutex> lock(asking);
+        allowSharedMemory<productTiles<128, 1, true, false, true>>(L::kBytes);
+        for (uint32_t i = 0; i < 3; ++i) {
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 2u << i, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t config{};
+            config.gridDim = dim3(8 * multiprocessors());
+            config.blockDim = dim3(L::kThreads);
+            config.dynamicSmemBytes = L::kBytes;
+            config.attrs = &attr;
+            config.numAttrs = 1;
+            int count = 0;
+            checkCudaCall(cudaOccupancyMaxActiveClusters(&count, productTiles<128, 1, true, false, true>, &config));
+            d.count[i] = uint32_t(count);
+        }
+        d.known.store(true, std::memory_order_release);
+    }
+    return d.count;
 }
 
 void launchProduct(const Product& p) {
@@ -923,14 +974,7 @@ void launchProduct(const Product& p) {
         return;
     }
     const uint64_t rowTiles = ceilDiv(p.m, 128u), sms = multiprocessors();
-    // Few tiles of 128 x 128: two to eight CTAs share each one's k, as many as there are SMs for and at
-    // least four blocks of k for each.
-    const uint64_t tiles = rowTiles * ceilDiv(p.n, 128u);
-    const uint32_t kBlocks = ceilDiv(p.k, kBlock);
-    uint32_t splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && kBlocks >= 8 * splits &&
-           blocksPerSplit(kBlocks, 2 * splits) * (2 * splits - 1) < kBlocks) // none is left without a block
-        splits *= 2;
+    const uint32_t splits = ctasPerTile(rowTiles * ceilDiv(p.n, 128u), ceilDiv(p.k, kBlock), sharingClusters());
     // One row of tiles of [n, k] weights runs as fast or faster in narrower tiles (128 x 4096 x 4096 11.1
     // us either way, 64 x 2048 x 8192 17.4 us against 20.4), two rows gain (256 x 4096 x 4096 18.0 -> 13.1
     // us), and so do [k, n] weights, which have no narrower tiles (128 x 4096 x 4096 14.4 -> 11.2 us).
@@ -961,6 +1005,14 @@ uint32_t matmulDeviceStatus(bool reset) { return denseStatus(reset); }
 } // namespace tcc
 
 extern "C" {
+
+// Test hook: the CTAs that share a tile (returned) and the first block of k of each, with the end behind the last.
+uint32_t tcc_test_product_parts(uint64_t tiles, uint32_t k_blocks, const uint32_t clusters[3], uint32_t first[9]) {
+    const uint32_t parts = tcc::ctasPerTile(tiles, k_blocks, {clusters[0], clusters[1], clusters[2]});
+    for (uint32_t i = 0; i <= parts; ++i)
+        first[i] = std::min(tcc::firstBlock(k_blocks, i, parts), k_blocks);
+    return parts;
+}
 
 int tcc_matmul_fp8_blocks(const void* a, int a_type, uint64_t a_stride, const uint8_t* a_scales, uint32_t a_block_rows,
                           const void* b, int b_type, uint64_t b_stride, const uint8_t* b_scales, uint32_t b_block_rows,

@@ -92,3 +92,23 @@ def test_weight_grad_long_sums(rows, n, k, ranges, dtype, pad):
     off = ((dw.double() - want).abs() / want).max()
     assert off <= limit, (float(off), limit)
     assert T.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("k", [1152, 3200, 4096, 4100, 4224, 8193, 8320])  # 9, 25, 32, 33, 33, 65 and 65 blocks
+def test_product_parts_of_any_length(k, layout):
+    """CTAs that share k, whose parts are unlike: every block counts once."""
+    m, n = 200, 500
+    a = positive(m, k, 0.5, 2.0, 1)
+    b = positive(n, k, 0.01, 0.12, 2) if layout == "nk" else positive(k, n, 0.01, 0.12, 2)
+    sa = torch.randint(125, 130, (m, -(-k // 128)), generator=torch.Generator().manual_seed(5)).to(torch.uint8).cuda()
+    sb = torch.randint(125, 130, (-(-b.shape[0] // 128), -(-b.shape[1] // 128)), generator=torch.Generator().manual_seed(6))
+    sb = sb.to(torch.uint8).cuda()
+    wide = D.values(b, sb, 128)
+    want = D.values(a, sa) @ (wide.t() if layout == "nk" else wide)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        y = torch.full((m, n), float("nan"), device="cuda", dtype=dtype)
+        T.matmul_fp8_blocks(a, sa, b, sb, y, b_layout=layout)
+        # up to 12 blocks in one accumulator, eight sums
+        assert ((y.double() - want).abs() <= (D.half_step(dtype) + 48 * D.U + 8 * 2.0 ** -24) * want).all(), dtype
+    assert T.device_status() == 0
