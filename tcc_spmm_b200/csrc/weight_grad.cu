@@ -86,10 +86,17 @@ template <typename T, int CG> struct GradTile {
     static constexpr int kCols = kBk + kStages * kACols;
     static constexpr int kEpilogueWarps = 8, kBWarp = 16, kLoadWarp = 24, kMmaWarp = 27;
     static constexpr int kThreads = 32 * 28;
-    // Registers: 72 per thread at launch; the warpgroups then share them out, 152 for the epilogue's
-    // 128 sums.
-    static constexpr int kRegs = 72, kRegsEpilogue = 152, kRegsA = 40, kRegsB = 40, kRegsIssue = 40;
-    static_assert(2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * kRegs, "the shares exceed the launch's registers");
+    // Registers: 72 per thread at launch (seven warpgroups); the warpgroups then share them out, 152 for the
+    // epilogue's 128 sums.
+    static constexpr int kRegsEpilogue = 152, kRegsA = 40, kRegsB = 40, kRegsIssue = 40;
+    // Whether a kernel that was built with `regs` registers per thread, which a launch rounds up to a multiple of 8,
+    // has the shares to give: a warpgroup would wait for ever for registers that the launch did not get.
+    static constexpr bool sharesFit(int regs) {
+        const int held = (regs + 7) / 8 * 8;
+        return kRegsA <= held && kRegsB <= held && kRegsIssue <= held && held <= kRegsEpilogue &&
+               2 * kRegsEpilogue + 2 * kRegsA + 2 * kRegsB + kRegsIssue <= 7 * held;
+    }
+    static_assert(sharesFit(65) && sharesFit(72) && !sharesFit(64) && !sharesFit(160), "shares of 72 registers per thread");
     static_assert(kRaw * kRawBytes >= 8 * 4096 && kCols <= 512 && kBytes <= 232448 && kBytes > 116 * 1024, "resources: one CTA per SM");
 };
 
@@ -750,14 +757,12 @@ template <typename T, int CG, bool TMA>
 void launchTiles(const GradArgs& g, const Plan& p, int type, cudaStream_t stream) {
     using L = GradTile<T, CG>;
     constexpr auto kernel = gradTiles<T, CG, TMA>;
-    // The kernel shares its launch's registers out anew and would wait for ever for ones that it
-    // did not get.
     static const int regs = [] {
         cudaFuncAttributes attr{};
         checkCudaCall(cudaFuncGetAttributes(&attr, gradTiles<T, CG, TMA>));
         return attr.numRegs;
     }();
-    if (regs != L::kRegs)
+    if (!L::sharesFit(regs))
         throw CudaError("weight_grad_int8 was built with an unexpected register count");
     const uint64_t grid = uint64_t(p.tilesN) * p.tilesK * p.splits * CG;
     require(grid <= 0x7FFFFFFFull, "too many output tiles for one call");
