@@ -273,10 +273,11 @@ def weight_grad_int8(grad_y, q, scales, grad_w, accumulate: bool = False, worksp
     if workspace is None:
         need = weight_grad_int8_workspace_size(rows, n, k)
         if need:
-            if isinstance(stream, int):
-                cuda = _torch.cuda
-                stream = cuda.ExternalStream(stream, device) if stream else cuda.default_stream(device)
-            with _torch.cuda.stream(stream):  # nothing for None: the current stream
+            cuda = _torch.cuda
+            if stream is not None and not isinstance(stream, cuda.Stream):  # a handle, or what holds one
+                handle = _stream_handle(stream)
+                stream = cuda.ExternalStream(handle, device) if handle else cuda.default_stream(device)
+            with cuda.stream(stream):  # nothing for None: the current stream
                 workspace = _torch.empty(need, dtype=_torch.uint8, device=grad_y.device)
     elif (not isinstance(workspace, _torch.Tensor) or workspace.get_device() != device or
           not workspace.is_contiguous()):
