@@ -334,7 +334,7 @@ int tcc_quantize_blocks_fp8(const void* x, int x_type, uint64_t x_stride, void* 
  * operands are e4m3 or e5m2 blocks along k; a [k x n] operand has blocks of 128 x 128. The sum is
  * accumulated in fp32 and rounded once to fp32, bf16 or fp16; bias (n floats) may be NULL. Fast
  * where both operands' rows start on 16 bytes (base and stride multiples of 16); other alignments
- * run on a slower kernel. */
+ * run on a kernel without tensor cores, a hundred times slower for large matrices. */
 int tcc_matmul_fp8_blocks(const void* a, int a_type, uint64_t a_stride, const uint8_t* a_scales,
                           uint32_t a_block_rows, const void* b, int b_type, uint64_t b_stride,
                           const uint8_t* b_scales, uint32_t b_block_rows, int b_layout,

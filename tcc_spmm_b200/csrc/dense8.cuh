@@ -140,7 +140,8 @@ __device__ __forceinline__ float int8At(uint32_t flipped, int i) {
 }
 
 // ---- activation functions -----------------------------------------------------------------------
-// All forms keep the relative accuracy of the left tail, which 1 + erf and 1 + tanh lose. They work
+// All forms keep the relative accuracy of the left tail, which 1 + erf and 1 + tanh lose, as far as the exponential
+// is a normal float. They work
 // on pairs, with the packed FP32 instructions (two lanes per issue) where there is a polynomial.
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
     return (uint64_t(__float_as_uint(b)) << 32) | __float_as_uint(a);
@@ -160,7 +161,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 // The hardware's approximations (2^-22 relative), results below 2^-126 as zero: without the steps
-// that keep subnormal results, which no rounding of the outputs could show.
+// that keep subnormal results. SiLU is zero below about -87 for it, where it is |x| 2^-126 and less.
 __device__ __forceinline__ float exp2Approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -135,7 +135,8 @@ template <typename T> void launchGeneric(const Product& p) {
 // a fixed order. The order of k in mma.m16n8k32 may be any that both operands share, so a lane reads 16
 // bytes of k of two rows of b and of MT rows of a at a time: two MMAs per 64 of k and 8 rows of a. The sum
 // over a block is multiplied by the two scales, powers of two (see Halves). 7.2 us for 1 x 4096 x 4096 out of
-// HBM (2.3 TB/s; 2.4 us of it launch and drain), 20.9 us for 1 x 8192 x 8192 (3.2 TB/s).
+// HBM (2.3 TB/s; 2.4 us of it launch and drain), 20.9 us for 1 x 8192 x 8192 (3.2 TB/s: its 512 CTAs are 1.73 rounds on
+// 296 places, and each begins with an empty ring).
 template <int MT_> struct Few {
     static constexpr int MT = MT_;
     static constexpr int kWarps = 8, kRows = 16;         // rows of b per CTA
@@ -975,9 +976,10 @@ void launchProduct(const Product& p) {
     }
     const uint64_t rowTiles = ceilDiv(p.m, 128u), sms = multiprocessors();
     const uint32_t splits = ctasPerTile(rowTiles * ceilDiv(p.n, 128u), ceilDiv(p.k, kBlock), sharingClusters());
-    // One row of tiles of [n, k] weights runs as fast or faster in narrower tiles (128 x 4096 x 4096 11.1
-    // us either way, 64 x 2048 x 8192 17.4 us against 20.4), two rows gain (256 x 4096 x 4096 18.0 -> 13.1
-    // us), and so do [k, n] weights, which have no narrower tiles (128 x 4096 x 4096 14.4 -> 11.2 us).
+    // One row of tiles of [n, k] weights runs as fast or faster in narrower tiles where those fill the SMs (128 x 4096
+    // x 4096 11.1 us either way, 64 x 2048 x 8192 17.4 us against 20.4; not measured for few columns, which leave most
+    // SMs idle), two rows gain (256 x 4096 x 4096 18.0 -> 13.1 us), and so do [k, n] weights, which have no narrower
+    // tiles (128 x 4096 x 4096 14.4 -> 11.2 us).
     if (splits > 1 && (p.kn || rowTiles > 1)) {
         p.kn ? launchTiles<128, 1, true, true>(p, splits) : launchTiles<128, 1, false, true>(p, splits);
         return;

@@ -18,15 +18,16 @@
 // One thread issues the MMAs.
 //
 // The tensor core cuts off what an addition shifts out below the accumulator's last bit, about
-// 1.5e-8 of the sum for every MMA (measured; 2.1e-5 after 1300), so the accumulator is emptied every
-// 60 MMAs into the fp32 registers of eight warps, which round to nearest. The MMAs wait meanwhile:
-// halves of the accumulator that take turns need MMAs of 128 columns, which ran at 91 cycles instead
-// of 64.
+// 1.5e-8 of the sum for every MMA (measured; 2.1e-5 after 1300; more where all terms have one sign), so
+// the accumulator is emptied every 60 MMAs into the fp32 registers of eight warps, which round to
+// nearest. The MMAs wait meanwhile: halves of the accumulator that take turns need MMAs of 128
+// columns, which ran at 91 cycles instead of 64.
 //
 // 8192 x 4096 x 2048 bf16 takes 129 us (1.07 PFLOP/s; 128 tiles on 74 pairs are two rounds for 1.73),
-// bound by shared memory's bandwidth (80 KB a stage and SM for 512 cycles of MMAs). 1M rows x 128 x 256
-// takes 106 us in bf16 (5.1 TB/s) and 177 to 220 us in fp32, whose three parts run at the power limit (SM
-// clock 1.2 GHz).
+// bound by shared memory's bandwidth in this layout (80 KB a stage and SM for 512 cycles of MMAs, 32 of
+// them for the widened q; as operand A, in tensor memory, it would take none of it, and dy no copy). 1M
+// rows x 128 x 256 takes 106 us in bf16 (5.1 TB/s) and 177 to 220 us in fp32, whose three parts run at the
+// power limit (SM clock 1.2 GHz).
 #include "dense8.cuh"
 #include "dense8_tc.cuh"
 

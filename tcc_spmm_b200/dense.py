@@ -157,7 +157,9 @@ def matmul_fp8_blocks(a, a_scales, b, b_scales, output, bias=None, b_layout: str
 
     a and b: float8_e4m3fn or float8_e5m2 blocks; the shapes of the scales tell blocks of a row from
     blocks of 128 x 128 (b [k, n] needs the latter). The sum is accumulated in fp32 and rounded once
-    to output's type (fp32, bf16 or fp16)."""
+    to output's type (fp32, bf16 or fp16). Rows of a or b that do not start on 16 bytes run on a
+    kernel without tensor cores, a hundred times slower for large matrices: give 8-bit operands a row
+    stride that is a multiple of 16."""
     if _torch is None:
         _load()
     layout = LAYOUTS.get(b_layout)
