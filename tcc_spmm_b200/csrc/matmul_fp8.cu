@@ -134,8 +134,8 @@ template <typename T> void launchGeneric(const Product& p) {
 // all of a 4096-wide row in flight at once), and their sums are added up in shared memory at the end, in
 // a fixed order. The order of k in mma.m16n8k32 may be any that both operands share, so a lane reads 16
 // bytes of k of two rows of b and of MT rows of a at a time: two MMAs per 64 of k and 8 rows of a. The sum
-// over a block is multiplied by the two scales, powers of two (see Halves). 7.2 us for 1 x 4096 x 4096 out of
-// HBM (2.3 TB/s; 2.4 us of it launch and drain), 20.9 us for 1 x 8192 x 8192 (3.2 TB/s: its 512 CTAs are 1.73 rounds on
+// over a block is multiplied by the two scales, powers of two (see Halves). 6.9 us for 1 x 4096 x 4096 out of
+// HBM (2.4 TB/s; 2.4 us of it launch and drain), 19.0 us for 1 x 8192 x 8192 (3.5 TB/s: its 512 CTAs are 1.73 rounds on
 // 296 places, and each begins with an empty ring).
 template <int MT_> struct Few {
     static constexpr int MT = MT_;
@@ -938,6 +938,8 @@ const uint32_t (&sharingClusters())[3] {
     if (!d.known.load(std::memory_order_acquire)) {
         using L = Tile<128, 1>;
         const std::lock_guard<std::mutex> lock(asking);
+        if (d.known.load(std::memory_order_relaxed))
+            return d.count;
         allowSharedMemory<productTiles<128, 1, true, false, true>>(L::kBytes);
         for (uint32_t i = 0; i < 3; ++i) {
             cudaLaunchAttribute attr{};
